@@ -417,6 +417,135 @@ int awa_dit_stack_set_profiling(awa_dit_stack* stack, int enabled);
 /* After a profiled run has completed: milliseconds of each block. */
 int awa_dit_stack_block_times(const awa_dit_stack* stack, float* block_ms);
 
+/* ---- key/value cache in pages: attention over tokens of earlier calls ---- */
+
+/* No counterpart in the reference, which attends over whole grids: for a long
+ * video restored as it arrives (text tokens first, then frame after frame), or
+ * a text model next to it. Keys and values of every sequence live in pages of
+ * page_tokens slots of caller-owned pools; a sequence's page table row names
+ * its pages in order. A call brings new rows of each sequence: with length L
+ * (the new rows included) and n new rows, row j has slot L - n + j. So one
+ * descriptor serves the append, the attention and the read of a step.
+ *
+ * Pools, [pages][kv_heads][page_tokens] rows of head_dim features:
+ *   AWA_KV_BF16: bf16.
+ *   AWA_KV_MXFP4: four bits a feature, e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6
+ *     and sign), the even feature in a byte's low half; and in k_scale /
+ *     v_scale, rows of head_dim / 32 bytes, the power of two 2^(byte - 127) of
+ *     each 32 features (255: the 32 are NaN). The append takes the least power
+ *     with which no value is above 7 (codes are the nearest, ties to the even
+ *     code; 6 to 7 gives 6), at least 2^-126.
+ *
+ * lengths, page_table, cu_rows and positions are device memory that the
+ * kernels read when they run, so a captured call follows what they hold then.
+ * What they hold is checked there, and told in *status (or-ed; the caller
+ * zeroes it; null: not told):
+ *   AWA_KV_BAD_PAGE: a needed page table entry is outside the pool. Appended
+ *     and read rows of such a page are left out, its slots are not visible.
+ *   AWA_KV_BAD_LENGTH: a length is negative, beyond the page table row, or
+ *     below the sequence's new rows; AWA_KV_BAD_ROWS: its rows in cu_rows are
+ *     out of order, beyond the blobs, or more than max_rows. Such a sequence
+ *     takes no part in the call.
+ * Table entries behind a sequence's length are not read. Sequences may share
+ * pages, but not append to one slot in one call (either row may win). Rows of
+ * blobs behind the last sequence's are left as they were. Nothing is
+ * allocated: every call can be captured into a graph. */
+#define AWA_KV_BF16 0
+#define AWA_KV_MXFP4 1
+#define AWA_KV_BAD_PAGE 1
+#define AWA_KV_BAD_LENGTH 2
+#define AWA_KV_BAD_ROWS 4
+
+typedef struct awa_kv_cache {
+    int format;        /* AWA_KV_* */
+    int pages;         /* pages of the pools */
+    int page_tokens;   /* slots a page: a power of two, 16 to 1024 */
+    int kv_heads;
+    int head_dim;      /* 64 or 128 */
+    int sequences;     /* 1 to 65535 */
+    int table_width;   /* entries of a page table row, up to 2^30 slots */
+    int table_stride;  /* ints from row to row */
+    void *k, *v;             /* 16-byte aligned */
+    void *k_scale, *v_scale; /* AWA_KV_MXFP4 */
+    const int* page_table;   /* [sequences][table_stride] */
+    const int* lengths;      /* [sequences], new rows included */
+    int* status;             /* or null */
+} awa_kv_cache;
+
+/* The new rows in the packed blobs: sequence s has rows [cu_rows[s],
+ * cu_rows[s + 1]) (device, sequences + 1 ints), at most max_rows. cu_rows null:
+ * max_rows each. */
+typedef struct awa_kv_rows {
+    const int* cu_rows;
+    int max_rows;
+} awa_kv_rows;
+
+/* Rotary positions: rope_dim features of a row, rope_dim / axes for each axis
+ * of a position; pair i of an axis turns by position * base^(-2 i / (rope_dim /
+ * axes)), or position * frequencies[i] (host array of rope_dim / axes / 2
+ * radians, copied). Pairs are neighbours (2 i, 2 i + 1) as in awa_mmrope, or
+ * with halves (i, i + rope_dim / 2), which needs one axis and rope_dim % 16 ==
+ * 0. The other features stay. Angles are exact to 2^-40 of a turn or better for every
+ * position below 2^24, and 2^-32 for every 32-bit one. */
+typedef struct awa_rope_desc {
+    int rope_dim; /* up to 128 */
+    int axes;     /* 1 to 4 */
+    int halves;
+    double base;
+    const double* frequencies; /* or null */
+} awa_rope_desc;
+
+typedef struct awa_rope awa_rope;
+
+int awa_rope_create(const awa_rope_desc* desc, awa_rope** rope);
+void awa_rope_destroy(awa_rope* rope);
+
+/* Appends new rows: k, rotated, and v into the pages (rounded once, to the
+ * cache's format); q, rotated, to q_out (q itself, or memory apart from it).
+ * Mats (head_dim, heads, rows) of one type, fp32 or bf16, rows (cstep) at
+ * 16-byte addresses, so views of a fused QKV projection will do. rope null:
+ * keys go in as they are and there is no q. positions: device ints
+ * [rows][axes], or null with one axis: the slot. */
+int awa_kv_append(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob* k, const awa_blob* v,
+                  const awa_rope* rope, const int* positions, const awa_blob* q, const awa_blob* q_out, void* stream);
+
+/* The last rows of each sequence out of the pages: row j of a sequence's n
+ * takes slot L - n + j, as the cache holds it (n = L: the whole sequence; for
+ * moving one elsewhere or to another format). */
+int awa_kv_read(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob* k_out, const awa_blob* v_out,
+                void* stream);
+
+/* What a row sees. The row at slot p sees keys below end(p) that are within
+ * the window before it or among the first `sinks` slots:
+ *   e = sinks + block * ceil((p + 1 - sinks) / block), end(p) = min(L, e),
+ *   visible: k < end(p) and (window == 0 or k >= e - window or k < sinks).
+ * block 1 is causal attention (e = p + 1). block > 1: blocks of that many
+ * slots behind the sinks see each other, as the tokens of a frame do.
+ * max_length: an upper bound of the lengths, 0 for all that a page table row
+ * can name. It sets how far the work is split; longer sequences are still
+ * right. */
+typedef struct awa_kv_mask {
+    int window; /* 0: unlimited */
+    int sinks;
+    int block;  /* at least 1 */
+    int max_length;
+} awa_kv_mask;
+
+/* out = softmax(scale q k^T) v over the keys that each new row sees, for q, out
+ * Mats (head_dim, heads, rows) of one type, heads a multiple of kv_heads (query
+ * head h reads key/value head h / (heads / kv_heads)). fp32 statistics and
+ * sums; bf16 rows round probabilities to bf16, fp32 rows keep 24 bits of
+ * queries and probabilities. A row that sees nothing gives zeros; what masked
+ * slots hold (NaN too) does not matter. out may be q.
+ * workspace: device memory of awa_kv_attention_workspace bytes for the same
+ * arguments, 16-byte aligned, for this call alone while it runs (calls on
+ * other streams, and captured graphs that may run beside each other, need
+ * their own). */
+int awa_kv_attention_workspace(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob* q,
+                               const awa_kv_mask* mask, size_t* bytes);
+int awa_kv_attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob* q, const awa_kv_mask* mask,
+                     float scale, const awa_blob* out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,11 @@ AWA_ERR_ALLOC = -100
 COMPUTE_F32 = 0  # exact-score fp32 kernel (int8 digit slices + bf16 pieces)
 COMPUTE_BF16 = 1
 COMPUTE_F32_MFMA = 2  # fp32 MFMA with plain accumulation (comparison path)
+KV_BF16 = 0  # pages of bf16
+KV_MXFP4 = 1  # pages of e2m1 codes, one power of two for each 32 features
+KV_BAD_PAGE = 1  # bits of a cache's status
+KV_BAD_LENGTH = 2
+KV_BAD_ROWS = 4
 
 # Every symbol of include/seedvr2_awa.h.
 EXPORTED_SYMBOLS = (
@@ -42,6 +47,8 @@ EXPORTED_SYMBOLS = (
     "awa_stack_block_flops", "awa_dit_block_create", "awa_dit_block_destroy", "awa_dit_block_forward",
     "awa_dit_stack_create", "awa_dit_stack_destroy", "awa_dit_stack_run", "awa_dit_stack_set_profiling",
     "awa_dit_stack_block_times",
+    "awa_rope_create", "awa_rope_destroy", "awa_kv_append", "awa_kv_read", "awa_kv_attention_workspace",
+    "awa_kv_attention",
 )
 
 
@@ -101,6 +108,29 @@ class AwaDitBranchWeights(ctypes.Structure):
     """awa_dit_branch_weights: device pointers of one branch's weights."""
     _fields_ = [(name, ctypes.c_void_p) for name in (
         "qkv", "proj_out", "proj_out_bias", "mlp_gate", "mlp_in", "mlp_out", "norm_q", "norm_k", "ada")]
+
+
+class AwaKvCache(ctypes.Structure):
+    """awa_kv_cache."""
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "format", "pages", "page_tokens", "kv_heads", "head_dim", "sequences", "table_width", "table_stride")] + [
+        (name, ctypes.c_void_p) for name in ("k", "v", "k_scale", "v_scale", "page_table", "lengths", "status")]
+
+
+class AwaKvRows(ctypes.Structure):
+    """awa_kv_rows."""
+    _fields_ = [("cu_rows", ctypes.c_void_p), ("max_rows", ctypes.c_int)]
+
+
+class AwaKvMask(ctypes.Structure):
+    """awa_kv_mask."""
+    _fields_ = [(name, ctypes.c_int) for name in ("window", "sinks", "block", "max_length")]
+
+
+class AwaRopeDesc(ctypes.Structure):
+    """awa_rope_desc."""
+    _fields_ = [(name, ctypes.c_int) for name in ("rope_dim", "axes", "halves")] + [
+        ("base", ctypes.c_double), ("frequencies", ctypes.POINTER(ctypes.c_double))]
 
 
 class AwaPlanInfo(ctypes.Structure):
@@ -179,6 +209,14 @@ def lib() -> ctypes.CDLL:
         L.awa_dit_stack_run.argtypes = [vp, wp, wp, vp, vp, vp, vp, vp, vp]
         L.awa_dit_stack_set_profiling.argtypes = [vp, i]
         L.awa_dit_stack_block_times.argtypes = [vp, ctypes.POINTER(ctypes.c_float)]
+        cp, rp, mp = ctypes.POINTER(AwaKvCache), ctypes.POINTER(AwaKvRows), ctypes.POINTER(AwaKvMask)
+        L.awa_rope_create.argtypes = [ctypes.POINTER(AwaRopeDesc), ctypes.POINTER(vp)]
+        L.awa_rope_destroy.argtypes = [vp]
+        L.awa_rope_destroy.restype = None
+        L.awa_kv_append.argtypes = [cp, rp, bp, bp, vp, vp, bp, bp, vp]
+        L.awa_kv_read.argtypes = [cp, rp, bp, bp, vp]
+        L.awa_kv_attention_workspace.argtypes = [cp, rp, bp, mp, ctypes.POINTER(sz)]
+        L.awa_kv_attention.argtypes = [cp, rp, bp, mp, ctypes.c_float, bp, vp, sz, vp]
         _LIB = L
     return _LIB
 
@@ -563,6 +601,78 @@ def qkv_concat(q: AwaBlob, k: AwaBlob, v: AwaBlob, out: AwaBlob, stream: Optiona
 
 def cast(inp: AwaBlob, out: AwaBlob, stream: Optional[Stream] = None) -> None:
     check(lib().awa_cast(ctypes.byref(inp), ctypes.byref(out), _s(stream)), "awa_cast")
+
+
+# ---- key/value cache in pages (pointers are device addresses) ----
+
+def KvCache(fmt: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int, k: int, v: int, page_table: int,
+            sequences: int, table_width: int, lengths: int, k_scale: int = 0, v_scale: int = 0, status: int = 0,
+            table_stride: int = 0) -> AwaKvCache:
+    """awa_kv_cache over the caller's pools, page table [sequences][table_width] and lengths."""
+    return AwaKvCache(fmt, pages, page_tokens, kv_heads, head_dim, sequences, table_width, table_stride or table_width,
+                      k or None, v or None, k_scale or None, v_scale or None, page_table or None, lengths or None,
+                      status or None)
+
+
+def KvRows(max_rows: int, cu_rows: int = 0) -> AwaKvRows:
+    """New rows a sequence: cu_rows [sequences + 1], or 0 for max_rows each."""
+    return AwaKvRows(cu_rows or None, max_rows)
+
+
+def KvMask(window: int = 0, sinks: int = 0, block: int = 1, max_length: int = 0) -> AwaKvMask:
+    return AwaKvMask(window, sinks, block, max_length)
+
+
+class Rope:
+    """Rotary positions (awa_rope_*)."""
+
+    def __init__(self, rope_dim: int, axes: int = 1, base: float = 10000.0, halves: bool = False,
+                 frequencies: Optional[Sequence[float]] = None):
+        freq = None
+        if frequencies is not None:
+            if axes < 1 or len(frequencies) != rope_dim // axes // 2:
+                raise ValueError("one frequency for each pair of an axis")
+            freq = (ctypes.c_double * len(frequencies))(*frequencies)
+        desc = AwaRopeDesc(rope_dim, axes, int(halves), base, freq)
+        p = ctypes.c_void_p()
+        check(lib().awa_rope_create(ctypes.byref(desc), ctypes.byref(p)), "awa_rope_create")
+        self.handle = p.value
+
+    def destroy(self) -> None:
+        if self.handle:
+            lib().awa_rope_destroy(ctypes.c_void_p(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+def kv_append(cache: AwaKvCache, rows: AwaKvRows, k: AwaBlob, v: AwaBlob, rope: Optional[Rope] = None,
+              positions: Optional[int] = None, q: Optional[AwaBlob] = None, q_out: Optional[AwaBlob] = None,
+              stream: Optional[Stream] = None) -> None:
+    check(lib().awa_kv_append(cache, rows, k, v, rope.handle if rope is not None else None, positions, q, q_out,
+                              _s(stream)), "awa_kv_append")
+
+
+def kv_read(cache: AwaKvCache, rows: AwaKvRows, k_out: AwaBlob, v_out: AwaBlob,
+            stream: Optional[Stream] = None) -> None:
+    check(lib().awa_kv_read(cache, rows, k_out, v_out, _s(stream)), "awa_kv_read")
+
+
+def kv_attention_workspace(cache: AwaKvCache, rows: AwaKvRows, q: AwaBlob, mask: AwaKvMask) -> int:
+    """Bytes of workspace that kv_attention needs for these arguments."""
+    n = ctypes.c_size_t()
+    check(lib().awa_kv_attention_workspace(cache, rows, q, mask, ctypes.byref(n)), "awa_kv_attention_workspace")
+    return n.value
+
+
+def kv_attention(cache: AwaKvCache, rows: AwaKvRows, q: AwaBlob, mask: AwaKvMask, scale: float, out: AwaBlob,
+                 workspace: Optional[int] = None, workspace_bytes: int = 0, stream: Optional[Stream] = None) -> None:
+    check(lib().awa_kv_attention(cache, rows, q, mask, scale, out, workspace, workspace_bytes, _s(stream)),
+          "awa_kv_attention")
 
 
 # ---- numpy helpers for bf16 bit patterns ----

@@ -1,0 +1,178 @@
+// Key/value cache in pages: the launch interface of its kernels (gfx950) and
+// the arithmetic that kernels and host checks share: which rows a sequence
+// brings, what a row sees, and how its keys are dealt out. Pointers are device
+// pointers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "seedvr2_awa.h"
+
+namespace awa
+{
+
+constexpr int kKvMaxSlots = 1 << 30; // slots a page table row may name
+constexpr int kKvGroup = 32;         // features that share a 4-bit row's power of two
+constexpr int kRopeMaxPairs = 64;
+
+struct KvView
+{
+    int pages, page_shift, heads; // key/value heads
+    unsigned char *k, *v, *k_scale, *v_scale;
+    const int* table;
+    int sequences, table_width, table_stride;
+    const int* lengths;
+    int* status;
+    // This call's new rows.
+    const int* cu;
+    int max_rows, total_rows;
+};
+
+// The new rows of one sequence: packed rows [first, first + rows), at slots
+// [length - rows, length). What does not fit together (bad != 0) has no rows,
+// so that nothing of it is read or written.
+struct KvSequence
+{
+    int first, rows, length;
+    unsigned bad;
+};
+
+__host__ __device__ inline KvSequence kv_sequence(int first, int end, int length, int capacity, int max_rows,
+                                                  int total_rows)
+{
+    KvSequence s{first, 0, length, 0u};
+    if (first < 0 || end < first || end > total_rows || end - first > max_rows)
+        s.bad |= AWA_KV_BAD_ROWS;
+    if (length < 0 || length > capacity || (!s.bad && end - first > length))
+        s.bad |= AWA_KV_BAD_LENGTH;
+    if (!s.bad)
+        s.rows = end - first;
+    return s;
+}
+
+__host__ __device__ inline KvSequence kv_sequence(const KvView& c, int s)
+{
+    const int first = c.cu ? c.cu[s] : s * c.max_rows;
+    const int end = c.cu ? c.cu[s + 1] : first + c.max_rows;
+    return kv_sequence(first, end, c.lengths[s], c.table_width << c.page_shift, c.max_rows, c.total_rows);
+}
+
+struct KvMaskRule
+{
+    int window, sinks, block;
+};
+
+// What the row at slot p of a sequence of `length` sees: keys [0, sinks) and
+// [begin, end), sinks <= begin <= end. All three grow with p.
+struct KvSpan
+{
+    int sinks, begin, end;
+};
+
+__host__ __device__ inline KvSpan kv_span(const KvMaskRule& m, int p, int length)
+{
+    long long e = static_cast<long long>(p) + 1;
+    if (m.block > 1)
+    {
+        // The end of the row's block; blocks are counted from slot `sinks`.
+        const int d = p + 1 - m.sinks;
+        const int q = d >= 0 ? (d + m.block - 1 < 0 ? d / m.block + (d % m.block != 0) : (d + m.block - 1) / m.block)
+                             : -(-d / m.block);
+        e = m.sinks + static_cast<long long>(q) * m.block;
+    }
+    KvSpan s;
+    s.end = static_cast<int>(e < length ? e : length);
+    const long long b = m.window > 0 && e > m.window ? e - m.window : 0;
+    s.begin = static_cast<int>(b < s.end ? b : s.end);
+    s.sinks = m.sinks < s.begin ? m.sinks : s.begin;
+    return s;
+}
+
+// The key tiles that rows from `first` to `last` (spans of the first and the
+// last row) see: tiles [0, sinks) and [begin, begin + rest).
+struct KvTiles
+{
+    int sinks, begin, rest;
+};
+
+__host__ __device__ inline KvTiles kv_tiles(const KvSpan& first, const KvSpan& last, int tile_shift)
+{
+    const int up = (1 << tile_shift) - 1;
+    KvTiles t;
+    t.sinks = (last.sinks + up) >> tile_shift;
+    t.begin = first.begin >> tile_shift;
+    if (t.begin < t.sinks)
+        t.begin = t.sinks;
+    const int end = (last.end + up) >> tile_shift;
+    t.rest = end > t.begin ? end - t.begin : 0;
+    return t;
+}
+
+// Part i of n of `tiles` tiles: [first, end).
+__host__ __device__ inline int kv_part(int tiles, int i, int n)
+{
+    return static_cast<int>(static_cast<long long>(tiles) * i / n);
+}
+
+// Rotation of the first rope_dim features of a row.
+struct KvRope
+{
+    // Turns a position, as a 64-bit fraction: the angle of position x is
+    // 2 pi (x * turns mod 2^64) / 2^64, exact for every 32-bit x.
+    unsigned long long turns[kRopeMaxPairs];
+    int pairs;      // pairs an axis
+    int axes;       // 0: no rotation
+    int halves;     // pair i is features i and i + pairs, else 2 i and 2 i + 1
+};
+
+struct KvRowsSource
+{
+    const unsigned char* data;
+    long long stride; // bytes from row to row
+};
+
+struct KvAppendLaunch
+{
+    KvView cache;
+    int head_dim, q_heads;
+    bool f32;  // type of q, k, v and q_out
+    bool four; // 4-bit pages
+    KvRowsSource q, k, v, q_out; // q.data null: none
+    const int* positions;        // null: the slot
+    KvRope rope;
+};
+hipError_t launch_kv_append(const KvAppendLaunch& p, hipStream_t stream);
+
+struct KvReadLaunch
+{
+    KvView cache;
+    int head_dim;
+    bool f32; // type of k and v
+    bool four;
+    KvRowsSource k, v;
+};
+hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t stream);
+
+struct KvAttentionLaunch
+{
+    KvView cache;
+    int head_dim, group; // query heads a key/value head
+    bool f32, four;
+    KvRowsSource q, out;
+    KvMaskRule mask;
+    float scale_log2; // softmax scale * log2 e
+    int splits;       // parts that the keys of a row tile are dealt to
+    // splits > 1: per part, packed row and query head the unnormalised row
+    // [D] relative to its maximum, then all (maximum, sum) pairs.
+    float* partial;
+};
+
+// Parts that the work is dealt to, and the bytes of its partial rows.
+int kv_attention_splits(const KvView& cache, int group, const KvMaskRule& mask, int max_length);
+size_t kv_attention_partial_bytes(const KvView& cache, int group, int head_dim, int splits);
+hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream);
+
+} // namespace awa
