@@ -31,5 +31,14 @@ __device__ __forceinline__ void four_values(unsigned word, float unit, float (&v
     v[4] = c[0] * unit, v[5] = c[1] * unit, v[6] = d[0] * unit, v[7] = d[1] * unit;
 }
 
+// The same as bf16, of which every such value is one.
+__device__ __forceinline__ uint4 four_bf16(unsigned word, float unit)
+{
+    return make_uint4(__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, unit, 0)),
+                      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, unit, 1)),
+                      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, unit, 2)),
+                      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, unit, 3)));
+}
+
 } // namespace dev
 } // namespace awa

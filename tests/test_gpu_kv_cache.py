@@ -453,17 +453,19 @@ def test_keys_that_are_not_finite(gpu):
     assert (np.abs(got[:2] - want) <= bound).all()
 
 
-def test_scales(gpu):
+@pytest.mark.parametrize("count", [3, 70])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scales(gpu, count, dtype):
     """Zero (the mean), negative and large scales."""
     rng = np.random.default_rng(23)
     cache = M.Cache("bf16", [77], 2, 64, 16)
     cache.upload()
-    q = new_rows(rng, [3], 2, 64, "f32")
+    q = new_rows(rng, [count], 2, 64, dtype)
     for scale in (0.0, -0.25, 20.0, 1e-30):
-        got = run_attention(cache, [3], q, "f32", scale=scale)
+        got = run_attention(cache, [count], q, dtype, scale=scale)
         k, _ = cache.rows("k", 0)
         v, _ = cache.rows("v", 0)
-        want, bound = M.attention(q, k * np.sign(scale or 1.0), v, 77, 0, 0, 1, abs(scale), "f32")
+        want, bound = M.attention(q, k * np.sign(scale or 1.0), v, 77, 0, 0, 1, abs(scale), dtype)
         assert (np.abs(got - want) <= bound).all(), scale
 
 
