@@ -454,28 +454,30 @@ __device__ __forceinline__ size_t uniform(size_t x)
     return static_cast<size_t>(hi) << 32 | lo;
 }
 
-// A tile of 128 NB rows, each wave NB blocks of 32; key tiles of 64 go through
-// LDS, which all waves read. Bound by the matrix cores, and next by what feeds
-// them: an operand read from LDS serves one MFMA where a wave has 32 rows, and
-// that alone is all of LDS's bandwidth, so a wave takes 64 rows where there
-// are that many.
+// A tile of 32 rows a wave, WAVES waves; key tiles of 64 go through LDS, which
+// all waves read. Bound by the matrix cores, and next by what feeds them: an
+// operand read from LDS serves one MFMA, so that MFMAs at full rate take all of
+// LDS's bandwidth. With eight waves two share a matrix core, and one's softmax
+// runs beside the other's products.
 //
 // S^T = K Q^T (32x32x16): lane (col = lane % 32, half = lane / 32) holds row
 // col's scores of keys 8 (i / 4) + 4 half + i % 4 of a 32-key block, i < 16;
 // eight of them in a row are, in that order, what the lane holds of the PV
 // product's operand P^T, and V^T is read in the same key order. A step takes a
-// block's softmax and its product with the values while the matrix cores work
-// on the scores of the next block.
-template <int D, int NB, bool F32, bool FOUR>
-__global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch p, int row_tiles)
+// block's softmax and its product with the values beside the scores of the next
+// block; operands are read half a step before they are used.
+template <int D, int WAVES, bool F32, bool FOUR>
+__global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const KvAttentionLaunch p, int row_tiles)
 {
     constexpr int kPieces = F32 ? 3 : 1;
-    constexpr int kRows = 128 * NB;
+    constexpr int kRows = 32 * WAVES;
+    constexpr int kThreads = 64 * WAVES;
     constexpr int kKeys = 64;
     constexpr int kC = D / 16;
     constexpr int kDb = D / 32;
     constexpr int kRowBytes = D * 2;
     constexpr int kTileBytes = kKeys * kRowBytes;
+    constexpr int kRowChunks = kRowBytes / 16;
     constexpr int kElem = F32 ? 4 : 2;
     constexpr float kGrow = 8.f;
     // Keys of this tile, the next and the one after; values of this and the next.
@@ -483,8 +485,9 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
     __shared__ __attribute__((aligned(1024))) unsigned char v_lds[2 * kTileBytes];
     // A tile's values as they are, where some are not finite, and which tile.
     __shared__ __attribute__((aligned(1024))) unsigned char raw_lds[kTileBytes];
-    __shared__ bf16x8 raw_weights[4][4 * NB * kPieces][64];
     __shared__ int raw_tile;
+    // Which of a tile's four 16-key blocks have no page; of tile t at t % 4.
+    __shared__ unsigned no_page[4];
 
     const KvView& c = p.cache;
     const int seq = blockIdx.y;
@@ -512,23 +515,21 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
     const KvSpan first = span_of(row0);
     const KvSpan last = span_of(min(row0 + kRows, rows) - 1);
 
-    // This wave's rows.
-    const int wave_row0 = row0 + wave * 32 * NB;
+    // This wave's rows (past the end: the last row again, not stored).
+    const int wave_row0 = row0 + wave * 32;
     const bool active = wave_row0 < rows;
     const KvSpan w_first = span_of(min(wave_row0, rows - 1));
-    const KvSpan w_last = span_of(min(wave_row0 + 32 * NB, rows) - 1);
-    KvSpan span[NB];
-    bf16x8 q[NB][kC][kPieces];
+    const KvSpan w_last = span_of(min(wave_row0 + 32, rows) - 1);
+    const int row = min(wave_row0 + col, rows - 1);
+    const int token = row / p.group;
+    const int q_head = head * p.group + row - token * p.group;
+    const KvSpan span = kv_span(p.mask, slot0 + token, s.length);
+    bf16x8 q[kC][kPieces];
     // (Not zero, whose product with the -inf of a masked score is NaN.)
     const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);
-#pragma unroll
-    for (int n = 0; n < NB; n++)
     {
-        const int row = min(wave_row0 + 32 * n + col, rows - 1);
-        const int token = row / p.group;
-        span[n] = kv_span(p.mask, slot0 + token, s.length);
         const unsigned char* src = p.q.data + static_cast<long long>(s.first + token) * p.q.stride +
-                                   static_cast<long long>(head * p.group + row - token * p.group) * D * kElem;
+                                   static_cast<long long>(q_head) * D * kElem;
 #pragma unroll
         for (int i = 0; i < kC; i++)
         {
@@ -548,148 +549,117 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
 #pragma unroll
                 for (int e = 0; e < 8; e++)
                     v[e] = -v[e];
-            split_bf16<kPieces>(v, q[n][i]);
+            split_bf16<kPieces>(v, q[i]);
         }
     }
 
     const KvTiles tiles = kv_tiles(first, last, 6);
-    const int count = tiles.sinks + tiles.rest;
-    const int t_begin = kv_part(count, split, p.splits);
-    const int t_end = kv_part(count, split + 1, p.splits);
+    const int t_begin = kv_part(tiles.sinks + tiles.rest, split, p.splits);
+    const int t_end = kv_part(tiles.sinks + tiles.rest, split + 1, p.splits);
+
+    // A wave loads kLoadRows rows of every tile, which lie in one 16-key block.
+    constexpr int kLoadRows = kKeys / WAVES;
+    const int load_row = wave * kLoadRows;
+    const int load_block = load_row >> 4;
     const int* const table = c.table + static_cast<long long>(seq) * c.table_stride;
     const int slot_mask = (1 << c.page_shift) - 1;
-
-    // A key tile: its first key, which of its four 16-key blocks have a page,
-    // and the pool row of this wave's.
-    struct Tile
-    {
-        int key0;
-        unsigned there;
-        size_t row;
-    };
     unsigned bad = 0;
-    auto look_up = [&](int i) {
-        Tile t;
-        t.key0 = (i < tiles.sinks ? i : tiles.begin + i - tiles.sinks) << 6;
-        t.there = 0;
-        t.row = 0;
-#pragma unroll
-        for (int b = 0; b < 4; b++)
+    auto tile_key = [&](int t) {
+        t = min(t, t_end - 1);
+        return (t < tiles.sinks ? t : tiles.begin + t - tiles.sinks) << 6;
+    };
+    // (Blocks behind the last key have the last key's page; their rows are
+    // masked.)
+    auto page_of = [&](int key0) { return table[min(key0 + 16 * load_block, last.end - 1) >> c.page_shift]; };
+    auto pool_row_of = [&](int t, int key0, int page) {
+        const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
+        if (!ok)
         {
-            const int key = t.key0 + 16 * b;
-            const bool in = key < last.end;
-            const int page = table[(in ? key : t.key0) >> c.page_shift];
-            const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
-            if (in && ok)
-                t.there |= 1u << b;
-            if (!ok)
-                bad = AWA_KV_BAD_PAGE;
-            if (b == wave)
-                t.row = (((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) + (key & slot_mask);
+            bad = AWA_KV_BAD_PAGE;
+            if (lane == 0)
+                atomicOr(&no_page[t & 3], 1u << load_block);
         }
-        t.row = uniform(t.row);
-        return t;
+        return uniform((((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) +
+                       ((key0 + load_row) & slot_mask));
     };
 
     // Where a 16-byte chunk of a row lies in LDS: chunks are permuted so that
     // both operands' reads touch all banks (K: 16 rows, one chunk each; V: four
     // rows, two chunks each).
-    auto k_chunk = [](int row, int chunk) { return chunk ^ (D == 128 ? row & 15 : (row >> 1) & 7); };
-    auto v_chunk = [](int row, int chunk) { return chunk ^ (D == 128 ? (row & 3) << 2 : (row & 2) << 1); };
-
-    constexpr int kLoads = 16 * kRowBytes / 1024; // loads of 1 KB for a wave's 16 rows
-    constexpr int kRowChunks = kRowBytes / 16;
+    auto k_chunk = [](int r, int chunk) { return chunk ^ (D == 128 ? r & 15 : (r >> 1) & 7); };
+    auto v_chunk = [](int r, int chunk) { return chunk ^ (D == 128 ? (r & 3) << 2 : (r & 2) << 1); };
+    constexpr int kLoads = (kLoadRows * kRowBytes + 1023) / 1024; // loads of 1 KB
     const uint32_t lds_k = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)k_lds));
     const uint32_t lds_v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)v_lds));
-    uint32_t k_off[kLoads], v_off[kLoads];
-#pragma unroll
-    for (int j = 0; j < kLoads; j++)
-    {
-        const int row = (j * 64 + lane) / kRowChunks;
-        k_off[j] = row * kRowBytes + k_chunk(row, lane % kRowChunks) * 16;
-        v_off[j] = row * kRowBytes + v_chunk(row, lane % kRowChunks) * 16;
-    }
-    // 4-bit pages: a thread's 32 features of a row, kept in registers until
-    // they are written to LDS as bf16.
+    const int l_row = lane / kRowChunks; // of the first KB; of KB j: + j * (64 / kRowChunks)
+    // 4-bit pages: a lane's 32 features of a row, kept in registers until they
+    // are written to LDS as bf16.
+    constexpr int kGroups = D / 32;
+    const int f_row = lane / kGroups;
+    const int f_group = lane % kGroups;
     uint4 k_codes, v_codes;
     unsigned k_byte, v_byte;
-    constexpr int kGroups = D / 32;
-    const int f_row = lane / kGroups; // of the wave's 16 rows
-    const int f_group = lane % kGroups;
-    const bool f_on = f_row < 16;
-    auto load_k = [&](const Tile& t, int slot) {
+    auto load_k = [&](size_t pool_row, int slot) {
         if (FOUR)
         {
-            const size_t row = t.row + (f_row & 15);
-            k_codes = *reinterpret_cast<const uint4*>(c.k + row * (D / 2) + 16 * f_group);
-            k_byte = c.k_scale[row * kGroups + f_group];
+            const size_t r = pool_row + (f_row & (kLoadRows - 1));
+            k_codes = *reinterpret_cast<const uint4*>(c.k + r * (D / 2) + 16 * f_group);
+            k_byte = c.k_scale[r * kGroups + f_group];
             return;
         }
-        const unsigned char* const base = c.k + t.row * kRowBytes;
+        const unsigned char* const base = c.k + pool_row * kRowBytes;
 #pragma unroll
         for (int j = 0; j < kLoads; j++)
-            load_to_lds(base, k_off[j], lds_k + slot * kTileBytes + wave * 16 * kRowBytes + j * 1024);
+            load_to_lds(base + j * 1024,
+                        l_row * kRowBytes +
+                            k_chunk(load_row + j * (64 / kRowChunks) + l_row, lane % kRowChunks) * 16,
+                        lds_k + slot * kTileBytes + load_row * kRowBytes + j * 1024);
     };
-    auto load_v = [&](const Tile& t, int slot) {
+    auto load_v = [&](size_t pool_row, int slot) {
         if (FOUR)
         {
-            const size_t row = t.row + (f_row & 15);
-            v_codes = *reinterpret_cast<const uint4*>(c.v + row * (D / 2) + 16 * f_group);
-            v_byte = c.v_scale[row * kGroups + f_group];
+            const size_t r = pool_row + (f_row & (kLoadRows - 1));
+            v_codes = *reinterpret_cast<const uint4*>(c.v + r * (D / 2) + 16 * f_group);
+            v_byte = c.v_scale[r * kGroups + f_group];
             return;
         }
-        const unsigned char* const base = c.v + t.row * kRowBytes;
+        const unsigned char* const base = c.v + pool_row * kRowBytes;
 #pragma unroll
         for (int j = 0; j < kLoads; j++)
-            load_to_lds(base, v_off[j], lds_v + slot * kTileBytes + wave * 16 * kRowBytes + j * 1024);
+            load_to_lds(base + j * 1024,
+                        l_row * kRowBytes +
+                            v_chunk(load_row + j * (64 / kRowChunks) + l_row, lane % kRowChunks) * 16,
+                        lds_v + slot * kTileBytes + load_row * kRowBytes + j * 1024);
     };
     auto store_four = [&](unsigned char* dst, const uint4& codes, unsigned byte, auto chunk_of) {
-        if (!f_on)
+        if (f_row >= kLoadRows)
             return;
         const float unit = four_unit(byte);
         const unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
-        const int row = wave * 16 + f_row;
+        const int r = load_row + f_row;
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            *reinterpret_cast<uint4*>(dst + row * kRowBytes + chunk_of(row, 4 * f_group + j) * 16) =
+            *reinterpret_cast<uint4*>(dst + r * kRowBytes + chunk_of(r, 4 * f_group + j) * 16) =
                 four_bf16(words[j], unit);
     };
 
-    f32x16 o[NB][kDb];
-    float row_max[NB], neg_max[NB], row_sum[NB];
+    f32x16 o[kDb];
 #pragma unroll
-    for (int n = 0; n < NB; n++)
-    {
-        row_max[n] = -INFINITY;
-        neg_max[n] = 0.f;
-        row_sum[n] = 0.f;
+    for (int d = 0; d < kDb; d++)
 #pragma unroll
-        for (int d = 0; d < kDb; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                o[n][d][i] = 0.f;
-    }
-    bf16x8 w[NB][2][kPieces]; // a block's weights
+        for (int i = 0; i < 16; i++)
+            o[d][i] = 0.f;
+    float row_max = -INFINITY, neg_max = 0.f, row_sum = 0.f;
+    bf16x8 w[2][kPieces]; // a block's weights
 
-    auto qk = [&](f32x16 (&x)[NB], int slot, int u) {
+    bf16x8 ka[kC], va[2][kDb];
+    auto read_k = [&](int slot, int u) {
         const unsigned char* const base = k_lds + slot * kTileBytes + (32 * u + col) * kRowBytes;
 #pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                x[n][i] = 0.f;
-#pragma unroll
         for (int i = 0; i < kC; i++)
-        {
-            const bf16x8 a = *reinterpret_cast<const bf16x8*>(base + k_chunk(col, 2 * i + half) * 16);
-#pragma unroll
-            for (int e = kPieces - 1; e >= 0; e--)
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-                    x[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[n][i][e], x[n], 0, 0, 0);
-        }
+            ka[i] = *reinterpret_cast<const bf16x8*>(base + k_chunk(col, 2 * i + half) * 16);
     };
-    auto pv = [&](int slot, int u) {
+    auto read_v = [&](int slot, int u) {
         const int g = (lane >> 4) & 1;
         const int r = lane & 15;
         const unsigned char* const base = v_lds + slot * kTileBytes + (32 * u + 4 * half + (r >> 2)) * kRowBytes;
@@ -702,91 +672,27 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
                                                 v_chunk(r >> 2, 4 * d + 2 * g + ((r & 3) >> 1)) * 16 + (r & 1) * 8;
                 const i16x4 lohi[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at)),
                                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 8 * kRowBytes))};
-                const bf16x8 a = __builtin_bit_cast(bf16x8, lohi);
-#pragma unroll
-                for (int e = kPieces - 1; e >= 0; e--)
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-                        o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w[n][j][e], o[n][d], 0, 0, 0);
+                va[j][d] = __builtin_bit_cast(bf16x8, lohi);
             }
     };
-    // Adds the values that are not finite, which the tile holds as zeros: only
-    // to rows that see them (a product with a zero weight would be NaN).
-    auto keep_weights = [&](int u) {
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int e = 0; e < kPieces; e++)
-                    raw_weights[wave][((u * NB + n) * 2 + j) * kPieces + e][lane] = w[n][j][e];
-    };
-    auto add_raw = [&]() {
-#pragma unroll 1
-        for (int key = 0; key < kKeys; key++)
-        {
-            // Which lanes and which of their sixteen scores of a block are this key's.
-            const int at = ((key >> 3) & 3) * 4 + (key & 3);
-            const int owner = ((key >> 2) & 1) * 32 + col;
-            const unsigned char* const v = raw_lds + key * kRowBytes;
-            float weight[NB];
-#pragma unroll
-            for (int n = 0; n < NB; n++)
-            {
-                weight[n] = 0.f;
-#pragma unroll
-                for (int e = kPieces - 1; e >= 0; e--)
-                    weight[n] += static_cast<float>(reinterpret_cast<const __bf16*>(
-                        &raw_weights[wave][(((key >> 5) * NB + n) * 2 + (at >> 3)) * kPieces + e][owner])[at & 7]);
-            }
-#pragma unroll
-            for (int d = 0; d < kDb; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-                {
-                    const uint2 v4 = *reinterpret_cast<const uint2*>(v + v_chunk(key, 4 * d + g) * 16 + half * 8);
-                    const float value[4] = {bf16_lo(v4.x), bf16_hi(v4.x), bf16_lo(v4.y), bf16_hi(v4.y)};
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (weight[n] != 0.f && !(fabsf(value[e]) < INFINITY))
-                                o[n][d][4 * g + e] = fmaf(weight[n], value[e], o[n][d][4 * g + e]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-        }
-    };
-    // Weights of one row block from its scores.
-    auto weigh = [&](const f32x16& x, int n) {
-        float y[16];
+    auto qk = [&](f32x16& x) {
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            y[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale, neg_max[n]));
+            x[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kC; i++)
+#pragma unroll
+            for (int e = kPieces - 1; e >= 0; e--)
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[i], q[i][e], x, 0, 0, 0);
+    };
+    auto pv = [&]() {
 #pragma unroll
         for (int j = 0; j < 2; j++)
-        {
-            float z[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                z[e] = y[8 * j + e];
-            split_bf16<kPieces>(z, w[n][j]);
-            if (F32)
-            {
+            for (int e = kPieces - 1; e >= 0; e--)
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    row_sum[n] += z[e];
-            }
-            else
-            {
-                const bf16x2 ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                {
-                    const bf16x2 pair = {w[n][j][0][2 * e], w[n][j][0][2 * e + 1]};
-                    row_sum[n] = __builtin_amdgcn_fdot2_f32_bf16(pair, ones, row_sum[n], false);
-                }
-            }
-        }
+                for (int d = 0; d < kDb; d++)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[j][d], w[j][e], o[d], 0, 0, 0);
     };
     auto top_of = [&](const f32x16& x) {
         float top = x[0];
@@ -795,31 +701,97 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
             top = fmaxf(top, x[i]);
         return max_xor32(top);
     };
+    // Weights from scores.
+    auto weigh = [&](const f32x16& x) {
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            y[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale, neg_max));
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+        {
+            float z[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                z[e] = y[8 * j + e];
+            split_bf16<kPieces>(z, w[j]);
+            if (F32)
+            {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    row_sum += z[e];
+            }
+            else
+            {
+                const bf16x2 ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                {
+                    const bf16x2 pair = {w[j][0][2 * e], w[j][0][2 * e + 1]};
+                    row_sum = __builtin_amdgcn_fdot2_f32_bf16(pair, ones, row_sum, false);
+                }
+            }
+        }
+    };
+    // The values that are not finite, which the tile holds as zeros, to the
+    // rows that see them (a product with a zero weight would be NaN); weights
+    // are positive, so what they weigh does not matter.
+    auto add_raw = [&](int key0, unsigned none) {
+#pragma unroll 1
+        for (int key = 0; key < kKeys; key++)
+        {
+            const int k = key0 + key;
+            const bool sees = !((none >> (key >> 4)) & 1u) && k < span.end && (k >= span.begin || k < span.sinks);
+#pragma unroll
+            for (int d = 0; d < kDb; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                {
+                    const uint2 v4 = *reinterpret_cast<const uint2*>(raw_lds + key * kRowBytes +
+                                                                     v_chunk(key, 4 * d + g) * 16 + half * 8);
+                    const float value[4] = {bf16_lo(v4.x), bf16_hi(v4.x), bf16_lo(v4.y), bf16_hi(v4.y)};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[d][4 * g + e] += sees && !(fabsf(value[e]) < INFINITY) ? value[e] : 0.f;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    };
 
-    Tile cur{}, next{}, after{};
-    f32x16 x[2][NB]; // scores of blocks 0 and 1 of a tile
-    float top[NB];
+    f32x16 x[2]; // scores of a tile's two blocks
+    float top = 0.f;
     auto wait = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // (LDS alone: the loads of the next tiles go on.)
     auto wait_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // The first keys of this tile and the two after it, the next one's pool row
+    // and the page of the one after that.
+    int key_now = 0, key_next = 0, key_after = 0, page_after = 0;
+    size_t row_next = 0;
     if (t_begin < t_end)
     {
-        if (tid == 0)
+        if (tid < 4)
+            no_page[tid] = 0u;
+        if (tid == 4)
             raw_tile = -1;
-        next = look_up(t_begin);
-        after = look_up(min(t_begin + 1, t_end - 1));
-        load_k(next, 0);
+        __syncthreads();
+        key_now = tile_key(t_begin);
+        key_next = tile_key(t_begin + 1);
+        key_after = tile_key(t_begin + 2);
+        const size_t row_now = pool_row_of(t_begin, key_now, page_of(key_now));
+        load_k(row_now, 0);
         if (FOUR)
             store_four(k_lds, k_codes, k_byte, k_chunk);
-        load_k(after, 1);
-        load_v(next, 0);
+        row_next = t_begin + 1 < t_end ? pool_row_of(t_begin + 1, key_next, page_of(key_next)) : row_now;
+        page_after = page_of(key_after);
+        load_k(row_next, 1);
+        load_v(row_now, 0);
         wait();
         if (active)
         {
-            qk(x[0], 0, 0);
-#pragma unroll
-            for (int n = 0; n < NB; n++)
-                top[n] = top_of(x[0][n]) * scale;
+            read_k(0, 0);
+            qk(x[0]);
+            read_k(0, 1);
+            top = top_of(x[0]) * scale;
         }
     }
     int k_slot = 0; // of tile t: (t - t_begin) % 3
@@ -829,9 +801,6 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
         const int k_slot1 = k_slot == 2 ? 0 : k_slot + 1;
         const int k_slot2 = k_slot == 0 ? 2 : k_slot - 1;
         const int v_slot = (t - t_begin) & 1;
-        cur = next;
-        next = after;
-        after = look_up(min(t + 2, t_end - 1));
         if (FOUR)
         {
             store_four(k_lds + k_slot1 * kTileBytes, k_codes, k_byte, k_chunk);
@@ -840,23 +809,32 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
         // This tile's values and the next one's keys are there, and all waves
         // are done with the slots that are loaded next.
         wait();
-        load_k(after, k_slot2);
-        load_v(next, 1 - v_slot);
+        load_v(row_next, 1 - v_slot);
+        if (t + 2 < t_end)
+        {
+            row_next = pool_row_of(t + 2, key_after, page_after);
+            load_k(row_next, k_slot2);
+        }
+        const unsigned none = no_page[t & 3];
+        if (tid == 0)
+            no_page[(t + 3) & 3] = 0u; // tile t - 1's, which nobody needs any more
+        const int key_third = tile_key(t + 3);
+        page_after = page_of(key_third);
         // Tiles that some row sees in part. What no row of the workgroup sees
         // becomes zeros, and so do values that are not finite.
         bool raw = false;
-        if (cur.there != 15u || !((cur.key0 >= last.begin && cur.key0 + kKeys <= first.end) ||
-                                  cur.key0 + kKeys <= first.sinks))
+        if (none != 0u ||
+            !((key_now >= last.begin && key_now + kKeys <= first.end) || key_now + kKeys <= first.sinks))
         {
             uint4* const v = reinterpret_cast<uint4*>(v_lds + v_slot * kTileBytes);
-            constexpr int kMine = kKeys * kRowChunks / 256;
+            constexpr int kMine = kKeys * kRowChunks / kThreads;
             bool fine = true;
 #pragma unroll
             for (int j = 0; j < kMine; j++)
             {
-                const int i = tid + j * 256;
-                const int key = cur.key0 + i / kRowChunks;
-                if (((cur.there >> (i / kRowChunks >> 4)) & 1u) && key < last.end &&
+                const int i = tid + j * kThreads;
+                const int key = key_now + i / kRowChunks;
+                if (!((none >> (i / kRowChunks >> 4)) & 1u) && key < last.end &&
                     (key >= first.begin || key < last.sinks))
                     fine = fine && finite8(v[i]);
                 else
@@ -871,117 +849,95 @@ __global__ __launch_bounds__(256, 1) void kv_tile_kernel(const KvAttentionLaunch
 #pragma unroll
                 for (int j = 0; j < kMine; j++)
                 {
-                    const uint4 y = v[tid + j * 256];
-                    reinterpret_cast<uint4*>(raw_lds)[tid + j * 256] = y;
-                    v[tid + j * 256] = only_finite8(y);
+                    const uint4 y = v[tid + j * kThreads];
+                    reinterpret_cast<uint4*>(raw_lds)[tid + j * kThreads] = y;
+                    v[tid + j * kThreads] = only_finite8(y);
                 }
                 wait_lds();
             }
         }
         if (active)
         {
+            const bool edge = none != 0u || !((key_now >= w_last.begin && key_now + kKeys <= w_first.end) ||
+                                              key_now + kKeys <= w_first.sinks);
 #pragma unroll
             for (int u = 0; u < 2; u++)
             {
-                const int key0 = cur.key0 + 32 * u;
-                const unsigned there = (cur.there >> (2 * u)) & 3u;
-                if (there != 3u || !((key0 >= w_last.begin && key0 + 32 <= w_first.end) || key0 + 32 <= w_first.sinks))
+                if (edge)
                 {
+                    const int key0 = key_now + 32 * u + 4 * half;
+                    const int end = span.end - key0, begin = span.begin - key0, sinks = span.sinks - key0;
 #pragma unroll
-                    for (int n = 0; n < NB; n++)
+                    for (int i = 0; i < 16; i++)
                     {
+                        const int key = 8 * (i >> 2) + (i & 3);
+                        const bool page = !((none >> (2 * u + (i >> 3))) & 1u);
+                        x[u][i] = page & (key < end) & ((key >= begin) | (key < sinks)) ? x[u][i] : -INFINITY;
+                    }
+                    top = top_of(x[u]);
+                    top = top == -INFINITY ? top : top * scale;
+                }
+                if (__any(top > row_max + kGrow))
+                {
+                    const float m = fmaxf(row_max, top);
+                    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
+                    row_max = m;
+                    neg_max = m == -INFINITY ? 0.f : -m;
+                    row_sum *= alpha;
+#pragma unroll
+                    for (int d = 0; d < kDb; d++)
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                        {
-                            const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
-                            const bool seen = ((there >> (i >> 3)) & 1u) && key < span[n].end &&
-                                              (key >= span[n].begin || key < span[n].sinks);
-                            x[u][n][i] = seen ? x[u][n][i] : -INFINITY;
-                        }
-                        top[n] = top_of(x[u][n]);
-                        top[n] = top[n] == -INFINITY ? top[n] : top[n] * scale;
-                    }
+                            o[d][i] *= alpha;
                 }
-                bool grow = false;
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-                    grow = grow || top[n] > row_max[n] + kGrow;
-                if (__any(grow))
-                {
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-                    {
-                        const float m = fmaxf(row_max[n], top[n]);
-                        const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max[n] - m);
-                        row_max[n] = m;
-                        neg_max[n] = m == -INFINITY ? 0.f : -m;
-                        row_sum[n] *= alpha;
-#pragma unroll
-                        for (int d = 0; d < kDb; d++)
-                        {
-#pragma unroll
-                            for (int i = 0; i < 16; i++)
-                                o[n][d][i] *= alpha;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                }
-                // Behind the last tile these are scores of stale keys; nobody takes them.
-                qk(x[1 - u], u == 0 ? k_slot : k_slot1, 1 - u);
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-                    weigh(x[u][n], n);
-                pv(v_slot, u);
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-                    top[n] = top_of(x[1 - u][n]) * scale;
-                if (raw)
-                    keep_weights(u);
+                // (Behind the last tile the scores are of stale keys; nobody
+                // takes them.)
+                read_v(v_slot, u);
+                __builtin_amdgcn_sched_barrier(0);
+                qk(x[1 - u]);
+                weigh(x[u]);
+                __builtin_amdgcn_sched_barrier(0);
+                read_k(k_slot1, u);
+                pv();
+                top = top_of(x[1 - u]) * scale;
             }
             if (raw)
-                add_raw();
+                add_raw(key_now, none);
         }
         k_slot = k_slot1;
+        key_now = key_next;
+        key_next = key_after;
+        key_after = key_third;
     }
     // No load of this wave may be on its way into LDS when it ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (bad && c.status && tid == 0)
+    if (bad && c.status && lane == 0)
         atomicOr(c.status, static_cast<int>(bad));
-    if (!active)
+    const float sum = sum_xor32(row_sum);
+    if (wave_row0 + col >= rows)
         return;
-
-#pragma unroll
-    for (int n = 0; n < NB; n++)
+    const long long at = s.first + token;
+    if (p.splits > 1)
     {
-        const float sum = sum_xor32(row_sum[n]);
-        const int row = wave_row0 + 32 * n + col;
-        if (row >= rows)
-            continue;
-        const int token = row / p.group;
-        const int q_head = head * p.group + row - token * p.group;
-        const long long at = s.first + token;
-        if (p.splits > 1)
+        const size_t heads = static_cast<size_t>(c.heads) * p.group;
+        const size_t all = static_cast<size_t>(c.total_rows) * heads;
+        const size_t i = split * all + at * heads + q_head;
+        store_o(p.partial + i * D, o, 1.f, half);
+        if (half == 0)
         {
-            const size_t heads = static_cast<size_t>(c.heads) * p.group;
-            const size_t all = static_cast<size_t>(c.total_rows) * heads;
-            const size_t i = split * all + at * heads + q_head;
-            store_o(p.partial + i * D, o[n], 1.f, half);
-            if (half == 0)
-            {
-                float* const st = p.partial + p.splits * all * D + i * 2;
-                st[0] = row_max[n];
-                st[1] = sum;
-            }
-            continue;
+            float* const st = p.partial + p.splits * all * D + i * 2;
+            st[0] = row_max;
+            st[1] = sum;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + at * p.out.stride +
-                                   static_cast<long long>(q_head) * D * kElem;
-        if (F32)
-            store_o(reinterpret_cast<float*>(dst), o[n], inv, half);
-        else
-            store_o(reinterpret_cast<uint16_t*>(dst), o[n], inv, half);
+        return;
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + at * p.out.stride +
+                               static_cast<long long>(q_head) * D * kElem;
+    if (F32)
+        store_o(reinterpret_cast<float*>(dst), o, inv, half);
+    else
+        store_o(reinterpret_cast<uint16_t*>(dst), o, inv, half);
 }
 
 // Joins the parts of a row: M = max m_i, out = sum 2^(m_i - M) o_i / sum
@@ -1059,9 +1015,9 @@ hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
     if (s.few)
         hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p, s.tiles);
     else if (F32 || s.rows == 128)
-        hipLaunchKernelGGL((kv_tile_kernel<D, 1, F32, FOUR>), grid, dim3(256), 0, stream, p, s.tiles);
+        hipLaunchKernelGGL((kv_tile_kernel<D, 4, F32, FOUR>), grid, dim3(256), 0, stream, p, s.tiles);
     else
-        hipLaunchKernelGGL((kv_tile_kernel<D, 2, false, FOUR>), grid, dim3(256), 0, stream, p, s.tiles);
+        hipLaunchKernelGGL((kv_tile_kernel<D, 8, false, FOUR>), grid, dim3(512), 0, stream, p, s.tiles);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1)
         return e;
