@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "awa_device.h"
 #include "kv_device.h"
@@ -30,7 +31,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
-constexpr int kRowTile = 16; // rows of kv_rows_kernel's tile
+constexpr int kRowTile = 16;   // rows of kv_rows_kernel's tile
+constexpr int kTileRows = 128; // of kv_tile_kernel's
 constexpr int kKeyTile = 32;
 constexpr int kKeyShift = 5;
 constexpr int kWaves = 4;
@@ -454,11 +456,66 @@ __device__ __forceinline__ size_t uniform(size_t x)
     return static_cast<size_t>(hi) << 32 | lo;
 }
 
-// A tile of 32 rows a wave, WAVES waves; key tiles of 64 go through LDS, which
-// all waves read. Bound by the matrix cores, and next by what feeds them: an
-// operand read from LDS serves one MFMA, so that MFMAs at full rate take all of
-// LDS's bandwidth. With eight waves two share a matrix core, and one's softmax
-// runs beside the other's products.
+// Workgroups go to the XCDs in turn; each has its own L2. Of every eight units
+// (a sequence's key/value head) an XCD takes one, so that the workgroups that
+// read the same keys at about the same time share an L2; the rest of the units
+// is dealt out part by part. Parts (of a unit's row tiles, those with the most
+// keys first) come in their order, for the long ones to start first: a period
+// of them holds `each` parts of every unit.
+struct TileDeal
+{
+    int units, parts, each, period, periods; // period: items of an XCD
+};
+
+__host__ inline TileDeal tile_deal(int units, int parts)
+{
+    TileDeal d{units, parts, 1, 0, 0};
+    while (units % 8 * d.each % 8)
+        d.each *= 2;
+    d.period = units * d.each / 8;
+    if (units % 8 == 0)
+        d.period = units / 8;
+    d.periods = (parts + d.each - 1) / d.each;
+    return d;
+}
+
+struct TileItem
+{
+    int unit; // < 0: none
+    int part;
+};
+
+__device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
+{
+    const int xcd = block & 7;
+    const int j = block >> 3;
+    const int q = j / d.period;
+    const int k = j - q * d.period;
+    const int whole = d.units >> 3;
+    TileItem t;
+    if (k < whole * d.each)
+    {
+        t.unit = k % whole * 8 + xcd;
+        t.part = q * d.each + k / whole;
+    }
+    else
+    {
+        const int i = (k - whole * d.each) * 8 + xcd;
+        const int left = d.units - whole * 8;
+        t.unit = whole * 8 + i % left;
+        t.part = q * d.each + i / left;
+    }
+    return t.part < d.parts ? t : TileItem{-1, 0};
+}
+
+// A tile of 128 rows, 32 a wave; key tiles of 64 go through LDS, which all
+// waves read. Bound by the matrix cores, and next by what feeds them: an operand
+// read from LDS serves one MFMA, so that MFMAs at full rate take all of LDS's
+// bandwidth. Two workgroups share a CU, so that one's softmax, waits and edges
+// run beside the other's products (16384 rows, 20 heads: 1557 us with one
+// workgroup of eight waves, whose barriers keep them in step, 1462 so; with four
+// waves of 64 rows, which halve the operand reads but leave a matrix core one
+// wave to be fed by, 1834).
 //
 // S^T = K Q^T (32x32x16): lane (col = lane % 32, half = lane / 32) holds row
 // col's scores of keys 8 (i / 4) + 4 half + i % 4 of a 32-key block, i < 16;
@@ -466,12 +523,12 @@ __device__ __forceinline__ size_t uniform(size_t x)
 // product's operand P^T, and V^T is read in the same key order. A step takes a
 // block's softmax and its product with the values beside the scores of the next
 // block; operands are read half a step before they are used.
-template <int D, int WAVES, bool F32, bool FOUR>
-__global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const KvAttentionLaunch p, int row_tiles)
+template <int D, bool F32, bool FOUR>
+__global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal)
 {
     constexpr int kPieces = F32 ? 3 : 1;
-    constexpr int kRows = 32 * WAVES;
-    constexpr int kThreads = 64 * WAVES;
+    constexpr int kRows = kTileRows;
+    constexpr int kThreads = 256;
     constexpr int kKeys = 64;
     constexpr int kC = D / 16;
     constexpr int kDb = D / 32;
@@ -480,28 +537,30 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
     constexpr int kRowChunks = kRowBytes / 16;
     constexpr int kElem = F32 ? 4 : 2;
     constexpr float kGrow = 8.f;
-    // Keys of this tile, the next and the one after; values of this and the next.
-    __shared__ __attribute__((aligned(1024))) unsigned char k_lds[3 * kTileBytes];
-    __shared__ __attribute__((aligned(1024))) unsigned char v_lds[2 * kTileBytes];
-    // A tile's values as they are, where some are not finite, and which tile.
-    __shared__ __attribute__((aligned(1024))) unsigned char raw_lds[kTileBytes];
+    // At tile t: keys of t + 1 to t + kAhead + 1 (those of t are in registers or
+    // multiplied) and values of t to t + kAhead.
+    constexpr int kAhead = F32 && !FOUR ? 2 : 1;
+    constexpr int kRing = kAhead + 1;
+    __shared__ __attribute__((aligned(1024))) unsigned char k_lds[kRing * kTileBytes];
+    __shared__ __attribute__((aligned(1024))) unsigned char v_lds[kRing * kTileBytes];
+    // The last tile with values that are not finite.
     __shared__ int raw_tile;
-    // Which of a tile's four 16-key blocks have no page; of tile t at t % 4.
-    __shared__ unsigned no_page[4];
+    // Which of a tile's four 16-key blocks have no page; of tile t at t % 8.
+    __shared__ unsigned no_page[8];
 
     const KvView& c = p.cache;
-    const int seq = blockIdx.y;
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31;
     const int half = lane >> 5;
-    // The row tiles with the most keys first.
-    int block = blockIdx.x;
-    const int split = block % p.splits;
-    block /= p.splits;
-    const int head = block % c.heads;
-    const int tile = row_tiles - 1 - block / c.heads;
+    const TileItem item = tile_item(deal, blockIdx.x);
+    if (item.unit < 0)
+        return;
+    const int seq = item.unit / c.heads;
+    const int head = item.unit - seq * c.heads;
+    const int split = item.part % p.splits;
+    const int tile = deal.parts / p.splits - 1 - item.part / p.splits;
 
     const KvSequence s = kv_sequence(c, seq);
     if (s.bad && c.status && tid == 0)
@@ -557,10 +616,9 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
     const int t_begin = kv_part(tiles.sinks + tiles.rest, split, p.splits);
     const int t_end = kv_part(tiles.sinks + tiles.rest, split + 1, p.splits);
 
-    // A wave loads kLoadRows rows of every tile, which lie in one 16-key block.
-    constexpr int kLoadRows = kKeys / WAVES;
+    // A wave loads one 16-key block of every tile.
+    constexpr int kLoadRows = 16;
     const int load_row = wave * kLoadRows;
-    const int load_block = load_row >> 4;
     const int* const table = c.table + static_cast<long long>(seq) * c.table_stride;
     const int slot_mask = (1 << c.page_shift) - 1;
     unsigned bad = 0;
@@ -570,14 +628,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
     };
     // (Blocks behind the last key have the last key's page; their rows are
     // masked.)
-    auto page_of = [&](int key0) { return table[min(key0 + 16 * load_block, last.end - 1) >> c.page_shift]; };
+    auto page_of = [&](int key0) { return table[min(key0 + load_row, last.end - 1) >> c.page_shift]; };
     auto pool_row_of = [&](int t, int key0, int page) {
         const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
         if (!ok)
         {
             bad = AWA_KV_BAD_PAGE;
             if (lane == 0)
-                atomicOr(&no_page[t & 3], 1u << load_block);
+                atomicOr(&no_page[t & 7], 1u << wave);
         }
         return uniform((((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) +
                        ((key0 + load_row) & slot_mask));
@@ -733,10 +791,11 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
             }
         }
     };
-    // The values that are not finite, which the tile holds as zeros, to the
-    // rows that see them (a product with a zero weight would be NaN); weights
-    // are positive, so what they weigh does not matter.
-    auto add_raw = [&](int key0, unsigned none) {
+    // A tile's values that are not finite, to the rows that see them; the tile
+    // then holds zeros for them (a product with the zero weight of a row that
+    // does not see them would be NaN). Weights are positive, so what they weigh
+    // does not matter.
+    auto add_raw = [&](const unsigned char* v, int key0, unsigned none) {
 #pragma unroll 1
         for (int key = 0; key < kKeys; key++)
         {
@@ -747,8 +806,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
 #pragma unroll
                 for (int g = 0; g < 4; g++)
                 {
-                    const uint2 v4 = *reinterpret_cast<const uint2*>(raw_lds + key * kRowBytes +
-                                                                     v_chunk(key, 4 * d + g) * 16 + half * 8);
+                    const uint2 v4 =
+                        *reinterpret_cast<const uint2*>(v + key * kRowBytes + v_chunk(key, 4 * d + g) * 16 + half * 8);
                     const float value[4] = {bf16_lo(v4.x), bf16_hi(v4.x), bf16_lo(v4.y), bf16_hi(v4.y)};
 #pragma unroll
                     for (int e = 0; e < 4; e++)
@@ -760,32 +819,52 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
 
     f32x16 x[2]; // scores of a tile's two blocks
     float top = 0.f;
-    auto wait = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // The latest N loads of the wave may still be on their way.
+    auto wait = [&](auto latest) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(latest)::value) : "memory");
+    };
+    using Latest = std::integral_constant<int, FOUR ? 0 : 2 * (kAhead - 1) * kLoads>;
+    using None = std::integral_constant<int, 0>;
     // (LDS alone: the loads of the next tiles go on.)
     auto wait_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // The first keys of this tile and the two after it, the next one's pool row
-    // and the page of the one after that.
-    int key_now = 0, key_next = 0, key_after = 0, page_after = 0;
-    size_t row_next = 0;
+    // At tile t: the first keys of tiles t to t + kAhead + 2, pool rows of t + 1
+    // to t + kAhead + 1, and the page of the last (read a tile ahead).
+    constexpr int kPool = kAhead + 1;
+    int key[kPool + 2];
+    size_t pool[kPool];
+    int page = 0;
     if (t_begin < t_end)
     {
-        if (tid < 4)
+        if (tid < 8)
             no_page[tid] = 0u;
-        if (tid == 4)
+        if (tid == 8)
             raw_tile = -1;
         __syncthreads();
-        key_now = tile_key(t_begin);
-        key_next = tile_key(t_begin + 1);
-        key_after = tile_key(t_begin + 2);
-        const size_t row_now = pool_row_of(t_begin, key_now, page_of(key_now));
-        load_k(row_now, 0);
+#pragma unroll
+        for (int i = 0; i <= kPool; i++)
+            key[i] = tile_key(t_begin + i);
+        int pages[kPool];
+#pragma unroll
+        for (int i = 0; i < kPool; i++)
+            pages[i] = page_of(key[i]);
+        page = page_of(key[kPool]);
+        const size_t now = pool_row_of(t_begin, key[0], pages[0]);
+#pragma unroll
+        for (int i = 0; i < kPool - 1; i++)
+            pool[i] = pool_row_of(t_begin + 1 + i, key[i + 1], pages[i + 1]);
+        load_k(now, 0);
         if (FOUR)
             store_four(k_lds, k_codes, k_byte, k_chunk);
-        row_next = t_begin + 1 < t_end ? pool_row_of(t_begin + 1, key_next, page_of(key_next)) : row_now;
-        page_after = page_of(key_after);
-        load_k(row_next, 1);
-        load_v(row_now, 0);
-        wait();
+        load_v(now, 0);
+        load_k(pool[0], 1);
+        if (!FOUR)
+#pragma unroll
+            for (int i = 0; i < kAhead - 1; i++)
+            {
+                load_v(pool[i], i + 1);
+                load_k(pool[i + 1], i + 2);
+            }
+        wait(None{});
         if (active)
         {
             read_k(0, 0);
@@ -794,48 +873,51 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
             top = top_of(x[0]) * scale;
         }
     }
-    int k_slot = 0; // of tile t: (t - t_begin) % 3
+    int slot = 0; // of tile t: (t - t_begin) % kRing
 #pragma unroll 1
     for (int t = t_begin; t < t_end; t++)
     {
-        const int k_slot1 = k_slot == 2 ? 0 : k_slot + 1;
-        const int k_slot2 = k_slot == 0 ? 2 : k_slot - 1;
-        const int v_slot = (t - t_begin) & 1;
+        const int slot1 = slot == kRing - 1 ? 0 : slot + 1;
+        const int key_now = key[0];
         if (FOUR)
         {
-            store_four(k_lds + k_slot1 * kTileBytes, k_codes, k_byte, k_chunk);
-            store_four(v_lds + v_slot * kTileBytes, v_codes, v_byte, v_chunk);
+            store_four(k_lds + slot1 * kTileBytes, k_codes, k_byte, k_chunk);
+            store_four(v_lds + slot * kTileBytes, v_codes, v_byte, v_chunk);
         }
         // This tile's values and the next one's keys are there, and all waves
-        // are done with the slots that are loaded next.
-        wait();
-        load_v(row_next, 1 - v_slot);
-        if (t + 2 < t_end)
+        // are done with the slots that are loaded next. (Behind the last tile
+        // the last is loaded again, so that the count of loads stays.)
+        wait(Latest{});
+        pool[kPool - 1] = pool_row_of(t + kPool, key[kPool], page);
+        if (FOUR)
         {
-            row_next = pool_row_of(t + 2, key_after, page_after);
-            load_k(row_next, k_slot2);
+            load_v(pool[0], 0);
+            load_k(pool[1], 0);
         }
-        const unsigned none = no_page[t & 3];
+        else
+        {
+            load_v(pool[kAhead - 1], slot == 0 ? kRing - 1 : slot - 1);
+            load_k(pool[kAhead], slot);
+        }
+        const unsigned none = no_page[t & 7];
         if (tid == 0)
-            no_page[(t + 3) & 3] = 0u; // tile t - 1's, which nobody needs any more
-        const int key_third = tile_key(t + 3);
-        page_after = page_of(key_third);
+            no_page[(t + kPool + 1) & 7] = 0u; // an earlier tile's, which nobody needs any more
+        key[kPool + 1] = tile_key(t + kPool + 1);
+        page = page_of(key[kPool + 1]);
         // Tiles that some row sees in part. What no row of the workgroup sees
         // becomes zeros, and so do values that are not finite.
-        bool raw = false;
         if (none != 0u ||
             !((key_now >= last.begin && key_now + kKeys <= first.end) || key_now + kKeys <= first.sinks))
         {
-            uint4* const v = reinterpret_cast<uint4*>(v_lds + v_slot * kTileBytes);
+            uint4* const v = reinterpret_cast<uint4*>(v_lds + slot * kTileBytes);
             constexpr int kMine = kKeys * kRowChunks / kThreads;
             bool fine = true;
 #pragma unroll
             for (int j = 0; j < kMine; j++)
             {
                 const int i = tid + j * kThreads;
-                const int key = key_now + i / kRowChunks;
-                if (!((none >> (i / kRowChunks >> 4)) & 1u) && key < last.end &&
-                    (key >= first.begin || key < last.sinks))
+                const int k = key_now + i / kRowChunks;
+                if (!((none >> (i / kRowChunks >> 4)) & 1u) && k < last.end && (k >= first.begin || k < last.sinks))
                     fine = fine && finite8(v[i]);
                 else
                     v[i] = make_uint4(0, 0, 0, 0);
@@ -843,16 +925,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
             if (!fine)
                 raw_tile = t;
             wait_lds();
-            raw = raw_tile == t;
-            if (raw)
+            if (raw_tile == t)
             {
+                if (active)
+                    add_raw(v_lds + slot * kTileBytes, key_now, none);
+                wait_lds();
 #pragma unroll
                 for (int j = 0; j < kMine; j++)
-                {
-                    const uint4 y = v[tid + j * kThreads];
-                    reinterpret_cast<uint4*>(raw_lds)[tid + j * kThreads] = y;
-                    v[tid + j * kThreads] = only_finite8(y);
-                }
+                    v[tid + j * kThreads] = only_finite8(v[tid + j * kThreads]);
                 wait_lds();
             }
         }
@@ -880,7 +960,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
                 if (__any(top > row_max + kGrow))
                 {
                     const float m = fmaxf(row_max, top);
-                    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
+                    // (Before the first weight there is nothing but what is not finite.)
+                    const float alpha = row_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
                     row_max = m;
                     neg_max = m == -INFINITY ? 0.f : -m;
                     row_sum *= alpha;
@@ -892,22 +973,23 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void kv_tile_kernel(const Kv
                 }
                 // (Behind the last tile the scores are of stale keys; nobody
                 // takes them.)
-                read_v(v_slot, u);
+                read_v(slot, u);
                 __builtin_amdgcn_sched_barrier(0);
                 qk(x[1 - u]);
                 weigh(x[u]);
                 __builtin_amdgcn_sched_barrier(0);
-                read_k(k_slot1, u);
+                read_k(slot1, u);
                 pv();
                 top = top_of(x[1 - u]) * scale;
             }
-            if (raw)
-                add_raw(key_now, none);
         }
-        k_slot = k_slot1;
-        key_now = key_next;
-        key_next = key_after;
-        key_after = key_third;
+        slot = slot1;
+#pragma unroll
+        for (int i = 0; i <= kPool; i++)
+            key[i] = key[i + 1];
+#pragma unroll
+        for (int i = 0; i < kPool - 1; i++)
+            pool[i] = pool[i + 1];
     }
     // No load of this wave may be on its way into LDS when it ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -989,7 +1071,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
 }
 
 // Row tiles: of 16 where no sequence has more than 32 rows a key/value head,
-// else of 128 or 256.
+// else of 128.
 struct Shape
 {
     bool few;
@@ -997,12 +1079,12 @@ struct Shape
     int tiles;
 };
 
-Shape shape_of(const KvView& c, int group, bool f32)
+Shape shape_of(const KvView& c, int group)
 {
     const long long rows = static_cast<long long>(c.max_rows) * group;
     Shape s;
     s.few = rows <= 32;
-    s.rows = s.few ? kRowTile : f32 || rows <= 128 ? 128 : 256;
+    s.rows = s.few ? kRowTile : kTileRows;
     s.tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
     return s;
 }
@@ -1010,14 +1092,17 @@ Shape shape_of(const KvView& c, int group, bool f32)
 template <int D, bool F32, bool FOUR>
 hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
 {
-    const Shape s = shape_of(p.cache, p.group, F32);
-    const dim3 grid(s.tiles * p.cache.heads * p.splits, p.cache.sequences);
+    const Shape s = shape_of(p.cache, p.group);
     if (s.few)
-        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p, s.tiles);
-    else if (F32 || s.rows == 128)
-        hipLaunchKernelGGL((kv_tile_kernel<D, 4, F32, FOUR>), grid, dim3(256), 0, stream, p, s.tiles);
+        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>),
+                           dim3(s.tiles * p.cache.heads * p.splits, p.cache.sequences), dim3(kWaves * 64), 0, stream, p,
+                           s.tiles);
     else
-        hipLaunchKernelGGL((kv_tile_kernel<D, 8, false, FOUR>), grid, dim3(512), 0, stream, p, s.tiles);
+    {
+        const TileDeal d = tile_deal(p.cache.heads * p.cache.sequences, s.tiles * p.splits);
+        const dim3 grid(8u * d.period * d.periods);
+        hipLaunchKernelGGL((kv_tile_kernel<D, F32, FOUR>), grid, dim3(256), 0, stream, p, d);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1)
         return e;
@@ -1029,9 +1114,9 @@ hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
 
 } // namespace
 
-int kv_attention_splits(const KvView& c, int group, bool f32, const KvMaskRule& mask, int max_length)
+int kv_attention_splits(const KvView& c, int group, const KvMaskRule& mask, int max_length)
 {
-    const Shape s = shape_of(c, group, f32);
+    const Shape s = shape_of(c, group);
     // Keys that a row tile may see, and the workgroups without splitting.
     long long keys = max_length;
     if (mask.window > 0)

@@ -144,7 +144,7 @@ int attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob
     const long long longest = mask->max_length > 0 && mask->max_length < slots ? mask->max_length : slots;
     if (static_cast<long long>(p.cache.max_rows) * q->h >= 1ll << 30)
         return invalid("max_rows times query heads must be below 2^30");
-    p.splits = awa::kv_attention_splits(p.cache, p.group, p.f32, p.mask, static_cast<int>(longest));
+    p.splits = awa::kv_attention_splits(p.cache, p.group, p.mask, static_cast<int>(longest));
     return AWA_OK;
 }
 

@@ -171,7 +171,7 @@ struct KvAttentionLaunch
 };
 
 // Parts that the work is dealt to, and the bytes of its partial rows.
-int kv_attention_splits(const KvView& cache, int group, bool f32, const KvMaskRule& mask, int max_length);
+int kv_attention_splits(const KvView& cache, int group, const KvMaskRule& mask, int max_length);
 size_t kv_attention_partial_bytes(const KvView& cache, int group, int head_dim, int splits);
 hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream);
 
