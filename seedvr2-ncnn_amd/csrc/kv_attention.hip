@@ -33,6 +33,8 @@ typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
 constexpr int kRowTile = 16;   // rows of kv_rows_kernel's tile
 constexpr int kTileRows = 128; // of kv_tile_kernel's
+constexpr int kTileShift = 5;  // and its keys
+constexpr int kTileKeys = 1 << kTileShift;
 constexpr int kKeyTile = 32;
 constexpr int kKeyShift = 5;
 constexpr int kWaves = 4;
@@ -416,6 +418,9 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
+// (Scalar loads: a vector load of a page would wait for the loads to LDS before
+// it.)
+typedef const __attribute__((address_space(4))) int constant_int;
 
 // 16 bytes a lane from base + offset to the 1 KB of LDS at `lds` (lane order);
 // the kernel waits for it itself. It has no output register.
@@ -508,28 +513,29 @@ __device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
     return t.part < d.parts ? t : TileItem{-1, 0};
 }
 
-// A tile of 128 rows, 32 a wave; key tiles of 64 go through LDS, which all
+// A tile of 128 rows, 32 a wave; key tiles of 32 go through LDS, which all
 // waves read. Bound by the matrix cores, and next by what feeds them: an operand
 // read from LDS serves one MFMA, so that MFMAs at full rate take all of LDS's
-// bandwidth. Two workgroups share a CU, so that one's softmax, waits and edges
-// run beside the other's products (16384 rows, 20 heads: 1557 us with one
-// workgroup of eight waves, whose barriers keep them in step, 1462 so; with four
-// waves of 64 rows, which halve the operand reads but leave a matrix core one
-// wave to be fed by, 1834).
+// bandwidth. Three workgroups share a CU (two of fp32 rows, whose queries take
+// three times the registers), so that one's softmax, waits and edges run beside
+// the others' products: nothing else of the loop overlaps by itself, and
+// schedules within a wave gained less. 16384 rows of 20 heads, 128 features: 1420
+// us so (950 TFLOP/s), 1426 with two workgroups that take the scores of the next
+// block beside a block's softmax, 1557 with one such of eight waves, whose
+// barriers keep them in step, 1834 with four waves of 64 rows, which read half
+// the operands but leave a matrix core one wave to be fed by.
 //
 // S^T = K Q^T (32x32x16): lane (col = lane % 32, half = lane / 32) holds row
-// col's scores of keys 8 (i / 4) + 4 half + i % 4 of a 32-key block, i < 16;
-// eight of them in a row are, in that order, what the lane holds of the PV
-// product's operand P^T, and V^T is read in the same key order. A step takes a
-// block's softmax and its product with the values beside the scores of the next
-// block; operands are read half a step before they are used.
+// col's scores of keys 8 (i / 4) + 4 half + i % 4, i < 16; eight of them in a row
+// are, in that order, what the lane holds of the PV product's operand P^T, and
+// V^T is read in the same key order.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal)
+__global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kRows = kTileRows;
     constexpr int kThreads = 256;
-    constexpr int kKeys = 64;
+    constexpr int kKeys = kTileKeys;
     constexpr int kC = D / 16;
     constexpr int kDb = D / 32;
     constexpr int kRowBytes = D * 2;
@@ -537,16 +543,13 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
     constexpr int kRowChunks = kRowBytes / 16;
     constexpr int kElem = F32 ? 4 : 2;
     constexpr float kGrow = 8.f;
-    // At tile t: keys of t + 1 to t + kAhead + 1 (those of t are in registers or
-    // multiplied) and values of t to t + kAhead.
-    constexpr int kAhead = F32 && !FOUR ? 2 : 1;
-    constexpr int kRing = kAhead + 1;
-    __shared__ __attribute__((aligned(1024))) unsigned char k_lds[kRing * kTileBytes];
-    __shared__ __attribute__((aligned(1024))) unsigned char v_lds[kRing * kTileBytes];
+    // Keys and values of this tile and the next.
+    __shared__ __attribute__((aligned(1024))) unsigned char k_lds[2][kTileBytes];
+    __shared__ __attribute__((aligned(1024))) unsigned char v_lds[2][kTileBytes];
     // The last tile with values that are not finite.
     __shared__ int raw_tile;
-    // Which of a tile's four 16-key blocks have no page; of tile t at t % 8.
-    __shared__ unsigned no_page[8];
+    // Which of a tile's two 16-key blocks have no page; of tile t at t % 4.
+    __shared__ unsigned no_page[4];
 
     const KvView& c = p.cache;
     const int tid = threadIdx.x;
@@ -612,19 +615,19 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
         }
     }
 
-    const KvTiles tiles = kv_tiles(first, last, 6);
+    const KvTiles tiles = kv_tiles(first, last, kTileShift);
     const int t_begin = kv_part(tiles.sinks + tiles.rest, split, p.splits);
     const int t_end = kv_part(tiles.sinks + tiles.rest, split + 1, p.splits);
 
-    // A wave loads one 16-key block of every tile.
-    constexpr int kLoadRows = 16;
+    // A wave loads half a 16-key block of every tile.
+    constexpr int kLoadRows = kKeys / 4;
     const int load_row = wave * kLoadRows;
-    const int* const table = c.table + static_cast<long long>(seq) * c.table_stride;
+    constant_int* const table = (constant_int*)(c.table + static_cast<long long>(seq) * c.table_stride);
     const int slot_mask = (1 << c.page_shift) - 1;
     unsigned bad = 0;
     auto tile_key = [&](int t) {
         t = min(t, t_end - 1);
-        return (t < tiles.sinks ? t : tiles.begin + t - tiles.sinks) << 6;
+        return (t < tiles.sinks ? t : tiles.begin + t - tiles.sinks) << kTileShift;
     };
     // (Blocks behind the last key have the last key's page; their rows are
     // masked.)
@@ -635,7 +638,7 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
         {
             bad = AWA_KV_BAD_PAGE;
             if (lane == 0)
-                atomicOr(&no_page[t & 7], 1u << wave);
+                atomicOr(&no_page[t & 3], 1u << (wave >> 1));
         }
         return uniform((((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) +
                        ((key0 + load_row) & slot_mask));
@@ -650,55 +653,46 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
     const uint32_t lds_k = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)k_lds));
     const uint32_t lds_v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)v_lds));
     const int l_row = lane / kRowChunks; // of the first KB; of KB j: + j * (64 / kRowChunks)
-    // 4-bit pages: a lane's 32 features of a row, kept in registers until they
-    // are written to LDS as bf16.
+    auto load = [&](size_t pool_row, int slot) {
+        const unsigned char* const k = c.k + pool_row * kRowBytes;
+        const unsigned char* const v = c.v + pool_row * kRowBytes;
+#pragma unroll
+        for (int j = 0; j < kLoads; j++)
+        {
+            const int r = j * (64 / kRowChunks) + l_row;
+            const uint32_t at = slot * kTileBytes + load_row * kRowBytes + j * 1024;
+            load_to_lds(k + j * 1024, l_row * kRowBytes + k_chunk(load_row + r, lane % kRowChunks) * 16, lds_k + at);
+            load_to_lds(v + j * 1024, l_row * kRowBytes + v_chunk(load_row + r, lane % kRowChunks) * 16, lds_v + at);
+        }
+    };
+    // 4-bit pages: a lane has 32 features of a key (the wave's first lanes) or of
+    // a value (the next ones), in registers until they go to LDS as bf16.
     constexpr int kGroups = D / 32;
-    const int f_row = lane / kGroups;
+    constexpr int kFourLanes = kLoadRows * kGroups;
     const int f_group = lane % kGroups;
-    uint4 k_codes, v_codes;
-    unsigned k_byte, v_byte;
-    auto load_k = [&](size_t pool_row, int slot) {
-        if (FOUR)
-        {
-            const size_t r = pool_row + (f_row & (kLoadRows - 1));
-            k_codes = *reinterpret_cast<const uint4*>(c.k + r * (D / 2) + 16 * f_group);
-            k_byte = c.k_scale[r * kGroups + f_group];
-            return;
-        }
-        const unsigned char* const base = c.k + pool_row * kRowBytes;
-#pragma unroll
-        for (int j = 0; j < kLoads; j++)
-            load_to_lds(base + j * 1024,
-                        l_row * kRowBytes +
-                            k_chunk(load_row + j * (64 / kRowChunks) + l_row, lane % kRowChunks) * 16,
-                        lds_k + slot * kTileBytes + load_row * kRowBytes + j * 1024);
+    const int f_row = lane / kGroups % kLoadRows;
+    const bool f_value = lane >= kFourLanes;
+    uint4 codes;
+    unsigned byte;
+    auto load_four = [&](size_t pool_row) {
+        const size_t r = pool_row + f_row;
+        codes = *reinterpret_cast<const uint4*>((f_value ? c.v : c.k) + r * (D / 2) + 16 * f_group);
+        byte = (f_value ? c.v_scale : c.k_scale)[r * kGroups + f_group];
     };
-    auto load_v = [&](size_t pool_row, int slot) {
-        if (FOUR)
-        {
-            const size_t r = pool_row + (f_row & (kLoadRows - 1));
-            v_codes = *reinterpret_cast<const uint4*>(c.v + r * (D / 2) + 16 * f_group);
-            v_byte = c.v_scale[r * kGroups + f_group];
-            return;
-        }
-        const unsigned char* const base = c.v + pool_row * kRowBytes;
-#pragma unroll
-        for (int j = 0; j < kLoads; j++)
-            load_to_lds(base + j * 1024,
-                        l_row * kRowBytes +
-                            v_chunk(load_row + j * (64 / kRowChunks) + l_row, lane % kRowChunks) * 16,
-                        lds_v + slot * kTileBytes + load_row * kRowBytes + j * 1024);
-    };
-    auto store_four = [&](unsigned char* dst, const uint4& codes, unsigned byte, auto chunk_of) {
-        if (f_row >= kLoadRows)
+    auto store_four = [&](int slot) {
+        if (lane >= 2 * kFourLanes)
             return;
         const float unit = four_unit(byte);
         const unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
         const int r = load_row + f_row;
+        unsigned char* const dst = (f_value ? v_lds[slot] : k_lds[slot]) + r * kRowBytes;
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            *reinterpret_cast<uint4*>(dst + r * kRowBytes + chunk_of(r, 4 * f_group + j) * 16) =
+        {
+            const int chunk = 4 * f_group + j;
+            *reinterpret_cast<uint4*>(dst + (f_value ? v_chunk(r, chunk) : k_chunk(r, chunk)) * 16) =
                 four_bf16(words[j], unit);
+        }
     };
 
     f32x16 o[kDb];
@@ -711,22 +705,20 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
     bf16x8 w[2][kPieces]; // a block's weights
 
     bf16x8 ka[kC], va[2][kDb];
-    auto read_k = [&](int slot, int u) {
-        const unsigned char* const base = k_lds + slot * kTileBytes + (32 * u + col) * kRowBytes;
+    auto read_k = [&](const unsigned char* k) {
 #pragma unroll
         for (int i = 0; i < kC; i++)
-            ka[i] = *reinterpret_cast<const bf16x8*>(base + k_chunk(col, 2 * i + half) * 16);
+            ka[i] = *reinterpret_cast<const bf16x8*>(k + col * kRowBytes + k_chunk(col, 2 * i + half) * 16);
     };
-    auto read_v = [&](int slot, int u) {
+    auto read_v = [&](const unsigned char* v) {
         const int g = (lane >> 4) & 1;
         const int r = lane & 15;
-        const unsigned char* const base = v_lds + slot * kTileBytes + (32 * u + 4 * half + (r >> 2)) * kRowBytes;
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
             for (int d = 0; d < kDb; d++)
             {
-                const unsigned char* const at = base + 16 * j * kRowBytes +
+                const unsigned char* const at = v + (16 * j + 4 * half + (r >> 2)) * kRowBytes +
                                                 v_chunk(r >> 2, 4 * d + 2 * g + ((r & 3) >> 1)) * 16 + (r & 1) * 8;
                 const i16x4 lohi[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at)),
                                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 8 * kRowBytes))};
@@ -817,99 +809,54 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
         }
     };
 
-    f32x16 x[2]; // scores of a tile's two blocks
-    float top = 0.f;
-    // The latest N loads of the wave may still be on their way.
-    auto wait = [&](auto latest) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(latest)::value) : "memory");
-    };
-    using Latest = std::integral_constant<int, FOUR ? 0 : 2 * (kAhead - 1) * kLoads>;
-    using None = std::integral_constant<int, 0>;
-    // (LDS alone: the loads of the next tiles go on.)
+    auto wait = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // (LDS alone: the loads of the next tile go on.)
     auto wait_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // At tile t: the first keys of tiles t to t + kAhead + 2, pool rows of t + 1
-    // to t + kAhead + 1, and the page of the last (read a tile ahead).
-    constexpr int kPool = kAhead + 1;
-    int key[kPool + 2];
-    size_t pool[kPool];
-    int page = 0;
+    // The first keys of this tile and the next, and the next one's page.
+    int key_now = 0, key_next = 0, page_next = 0;
     if (t_begin < t_end)
     {
-        if (tid < 8)
+        if (tid < 4)
             no_page[tid] = 0u;
-        if (tid == 8)
+        if (tid == 4)
             raw_tile = -1;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i <= kPool; i++)
-            key[i] = tile_key(t_begin + i);
-        int pages[kPool];
-#pragma unroll
-        for (int i = 0; i < kPool; i++)
-            pages[i] = page_of(key[i]);
-        page = page_of(key[kPool]);
-        const size_t now = pool_row_of(t_begin, key[0], pages[0]);
-#pragma unroll
-        for (int i = 0; i < kPool - 1; i++)
-            pool[i] = pool_row_of(t_begin + 1 + i, key[i + 1], pages[i + 1]);
-        load_k(now, 0);
+        key_now = tile_key(t_begin);
+        key_next = tile_key(t_begin + 1);
+        const size_t row_now = pool_row_of(t_begin, key_now, page_of(key_now));
+        page_next = page_of(key_next);
         if (FOUR)
-            store_four(k_lds, k_codes, k_byte, k_chunk);
-        load_v(now, 0);
-        load_k(pool[0], 1);
-        if (!FOUR)
-#pragma unroll
-            for (int i = 0; i < kAhead - 1; i++)
-            {
-                load_v(pool[i], i + 1);
-                load_k(pool[i + 1], i + 2);
-            }
-        wait(None{});
-        if (active)
-        {
-            read_k(0, 0);
-            qk(x[0]);
-            read_k(0, 1);
-            top = top_of(x[0]) * scale;
-        }
+            load_four(row_now);
+        else
+            load(row_now, 0);
     }
-    int slot = 0; // of tile t: (t - t_begin) % kRing
 #pragma unroll 1
     for (int t = t_begin; t < t_end; t++)
     {
-        const int slot1 = slot == kRing - 1 ? 0 : slot + 1;
-        const int key_now = key[0];
+        const int slot = (t - t_begin) & 1;
+        unsigned char* const k_tile = k_lds[slot];
+        unsigned char* const v_tile = v_lds[slot];
         if (FOUR)
-        {
-            store_four(k_lds + slot1 * kTileBytes, k_codes, k_byte, k_chunk);
-            store_four(v_lds + slot * kTileBytes, v_codes, v_byte, v_chunk);
-        }
-        // This tile's values and the next one's keys are there, and all waves
-        // are done with the slots that are loaded next. (Behind the last tile
-        // the last is loaded again, so that the count of loads stays.)
-        wait(Latest{});
-        pool[kPool - 1] = pool_row_of(t + kPool, key[kPool], page);
+            store_four(slot);
+        // This tile is there, and all waves are done with the one before.
+        // (Behind the last tile the last is loaded again.)
+        wait();
+        const size_t row_next = pool_row_of(t + 1, key_next, page_next);
         if (FOUR)
-        {
-            load_v(pool[0], 0);
-            load_k(pool[1], 0);
-        }
+            load_four(row_next);
         else
-        {
-            load_v(pool[kAhead - 1], slot == 0 ? kRing - 1 : slot - 1);
-            load_k(pool[kAhead], slot);
-        }
-        const unsigned none = no_page[t & 7];
+            load(row_next, 1 - slot);
+        const unsigned none = no_page[t & 3];
         if (tid == 0)
-            no_page[(t + kPool + 1) & 7] = 0u; // an earlier tile's, which nobody needs any more
-        key[kPool + 1] = tile_key(t + kPool + 1);
-        page = page_of(key[kPool + 1]);
+            no_page[(t + 2) & 3] = 0u; // tile t - 2's, which nobody needs any more
+        const int key_third = tile_key(t + 2);
+        page_next = page_of(key_third);
         // Tiles that some row sees in part. What no row of the workgroup sees
         // becomes zeros, and so do values that are not finite.
         if (none != 0u ||
             !((key_now >= last.begin && key_now + kKeys <= first.end) || key_now + kKeys <= first.sinks))
         {
-            uint4* const v = reinterpret_cast<uint4*>(v_lds + slot * kTileBytes);
+            uint4* const v = reinterpret_cast<uint4*>(v_tile);
             constexpr int kMine = kKeys * kRowChunks / kThreads;
             bool fine = true;
 #pragma unroll
@@ -928,7 +875,7 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
             if (raw_tile == t)
             {
                 if (active)
-                    add_raw(v_lds + slot * kTileBytes, key_now, none);
+                    add_raw(v_tile, key_now, none);
                 wait_lds();
 #pragma unroll
                 for (int j = 0; j < kMine; j++)
@@ -938,58 +885,45 @@ __global__ __launch_bounds__(256, F32 ? 1 : 2) void kv_tile_kernel(const KvAtten
         }
         if (active)
         {
-            const bool edge = none != 0u || !((key_now >= w_last.begin && key_now + kKeys <= w_first.end) ||
-                                              key_now + kKeys <= w_first.sinks);
-#pragma unroll
-            for (int u = 0; u < 2; u++)
+            read_k(k_tile);
+            f32x16 x;
+            qk(x);
+            float top = top_of(x) * scale;
+            if (none != 0u || !((key_now >= w_last.begin && key_now + kKeys <= w_first.end) ||
+                                key_now + kKeys <= w_first.sinks))
             {
-                if (edge)
+                const int key0 = key_now + 4 * half;
+                const int end = span.end - key0, begin = span.begin - key0, sinks = span.sinks - key0;
+#pragma unroll
+                for (int i = 0; i < 16; i++)
                 {
-                    const int key0 = key_now + 32 * u + 4 * half;
-                    const int end = span.end - key0, begin = span.begin - key0, sinks = span.sinks - key0;
+                    const int key = 8 * (i >> 2) + (i & 3);
+                    const bool page = !((none >> (i >> 3)) & 1u);
+                    x[i] = page & (key < end) & ((key >= begin) | (key < sinks)) ? x[i] : -INFINITY;
+                }
+                top = top_of(x);
+                top = top == -INFINITY ? top : top * scale;
+            }
+            if (__any(top > row_max + kGrow))
+            {
+                const float m = fmaxf(row_max, top);
+                // (Before the first weight there is nothing but what is not finite.)
+                const float alpha = row_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
+                row_max = m;
+                neg_max = m == -INFINITY ? 0.f : -m;
+                row_sum *= alpha;
+#pragma unroll
+                for (int d = 0; d < kDb; d++)
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                    {
-                        const int key = 8 * (i >> 2) + (i & 3);
-                        const bool page = !((none >> (2 * u + (i >> 3))) & 1u);
-                        x[u][i] = page & (key < end) & ((key >= begin) | (key < sinks)) ? x[u][i] : -INFINITY;
-                    }
-                    top = top_of(x[u]);
-                    top = top == -INFINITY ? top : top * scale;
-                }
-                if (__any(top > row_max + kGrow))
-                {
-                    const float m = fmaxf(row_max, top);
-                    // (Before the first weight there is nothing but what is not finite.)
-                    const float alpha = row_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
-                    row_max = m;
-                    neg_max = m == -INFINITY ? 0.f : -m;
-                    row_sum *= alpha;
-#pragma unroll
-                    for (int d = 0; d < kDb; d++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            o[d][i] *= alpha;
-                }
-                // (Behind the last tile the scores are of stale keys; nobody
-                // takes them.)
-                read_v(slot, u);
-                __builtin_amdgcn_sched_barrier(0);
-                qk(x[1 - u]);
-                weigh(x[u]);
-                __builtin_amdgcn_sched_barrier(0);
-                read_k(slot1, u);
-                pv();
-                top = top_of(x[1 - u]) * scale;
+                        o[d][i] *= alpha;
             }
+            read_v(v_tile);
+            weigh(x);
+            pv();
         }
-        slot = slot1;
-#pragma unroll
-        for (int i = 0; i <= kPool; i++)
-            key[i] = key[i + 1];
-#pragma unroll
-        for (int i = 0; i < kPool - 1; i++)
-            pool[i] = pool[i + 1];
+        key_now = key_next;
+        key_next = key_third;
     }
     // No load of this wave may be on its way into LDS when it ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
