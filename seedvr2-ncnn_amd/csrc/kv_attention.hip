@@ -81,23 +81,62 @@ __device__ __forceinline__ void store_o(T* dst, const f32x16 (&o)[N], float by, 
                    o[d][4 * g + 3] * by);
 }
 
-// One row tile of 16 rows, one part of its keys: each of the four waves takes
-// every fourth key tile (32 keys) by itself, with K from memory straight into
-// the MFMA operand registers and V through the wave's own LDS, from which it
-// is read transposed; the waves' results are joined at the end. Bound by
-// reading the cache.
+typedef __attribute__((address_space(3))) char lds_char;
+// (Scalar loads: a vector load of a page would wait for the loads to LDS before
+// it.)
+typedef const __attribute__((address_space(4))) int constant_int;
+
+// A value that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ size_t uniform(size_t x)
+{
+    const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
+    const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
+    return static_cast<size_t>(hi) << 32 | lo;
+}
+
+// Whether eight bf16 values are finite, and the finite ones of them (else 0).
+__device__ __forceinline__ bool finite8(const uint4& v)
+{
+    const unsigned words[4] = {v.x, v.y, v.z, v.w};
+    unsigned most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        most = max(most, max(words[e] & 0x7fffu, (words[e] >> 16) & 0x7fffu));
+    return most < 0x7f80u;
+}
+
+__device__ __forceinline__ uint4 only_finite8(const uint4& v)
+{
+    unsigned words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+    {
+        words[e] = (words[e] & 0x7f80u) == 0x7f80u ? words[e] & 0xffff0000u : words[e];
+        words[e] = (words[e] & 0x7f800000u) == 0x7f800000u ? words[e] & 0xffffu : words[e];
+    }
+    return make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+// One row tile of 16 rows, one part of its keys: each wave takes every fourth
+// key tile (32 keys) by itself, with K from memory straight into the MFMA
+// operand registers and V through the wave's own LDS, from which it is read
+// transposed; the waves' results are joined at the end. Bound by reading the
+// cache: the next tile's rows are asked for as soon as this one's registers are
+// free.
 //
 // S^T = K Q^T (16x16x32): lane (r = lane % 16, g = lane / 16) holds row r's
 // scores of keys 4 g + [0, 4) of each 16. Those of two blocks are, in that
 // order, the eight values a lane holds of the PV product's operand P^T; V^T is
-// read in the same key order.
+// read in the same key order. Which features an MFMA takes of a row does not
+// matter as long as both operands agree: of 4-bit rows a lane has a quarter,
+// one load and one scale.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p, int row_tiles)
+__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p, int row_tiles, int part_tiles)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kChunks = D / 32;
     constexpr int kBlocks = D / 16;
-    constexpr int kPitch = D + 32; // V rows in LDS, elements
+    constexpr int kPitch = D + 16; // V rows in LDS, elements: eight rows' reads touch all banks
     constexpr int kElem = F32 ? 4 : 2;
     constexpr int kVBytes = kKeyTile * kPitch * 2;
     constexpr int kOBytes = kRowTile * D * 4;
@@ -127,6 +166,13 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     const int slot0 = s.length - s.rows;
     const KvSpan span_first = kv_span(p.mask, slot0 + row0 / p.group, s.length);
     const KvSpan span_last = kv_span(p.mask, slot0 + last / p.group, s.length);
+    const KvTiles tiles = kv_tiles(span_first, span_last, kKeyShift);
+    const int count = tiles.sinks + tiles.rest;
+    // (The first part joins in for rows that see nothing.)
+    if (split * part_tiles >= count && split > 0)
+        return;
+    // (The last one takes all that is left: lengths may pass their bound.)
+    const int part_end = split + 1 == p.splits ? count : min(count, (split + 1) * part_tiles);
 
     // This lane's row (rows past the end repeat the last; they are not stored).
     const int row = min(row0 + r, last);
@@ -140,7 +186,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
 #pragma unroll
         for (int i = 0; i < kChunks; i++)
         {
-            const int feature = 32 * i + 8 * g;
+            const int feature = FOUR ? D / 4 * g + 8 * i : 32 * i + 8 * g;
             float v[8];
             uint32_t w[8];
             if (F32)
@@ -157,9 +203,86 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
         }
     }
 
-    const KvTiles tiles = kv_tiles(span_first, span_last, kKeyShift);
-    const int count = tiles.sinks + tiles.rest;
-    const int part_end = kv_part(count, split + 1, p.splits);
+    constant_int* const table = (constant_int*)(c.table + static_cast<long long>(seq) * c.table_stride);
+    const int slot_mask = (1 << c.page_shift) - 1;
+    unsigned bad = 0;
+    // A key tile: its first key, which of its two 16-key blocks are there, and
+    // their pool rows.
+    struct Tile
+    {
+        int key0;
+        unsigned there;
+        size_t base[2];
+    };
+    auto look_up = [&](int i) {
+        Tile t;
+        t.key0 = (i < tiles.sinks ? i : tiles.begin + i - tiles.sinks) << kKeyShift;
+        t.there = 0;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+        {
+            const int key = t.key0 + 16 * b;
+            const int page = table[min(key, span_last.end - 1) >> c.page_shift];
+            const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
+            if (ok && key < span_last.end)
+                t.there |= 1u << b;
+            if (!ok)
+                bad = AWA_KV_BAD_PAGE;
+            t.base[b] =
+                uniform((((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) + (key & slot_mask));
+        }
+        return t;
+    };
+
+    // K: lane r of block b has key 16 b + r. V: kVLanes lanes a row.
+    constexpr int kVLanes = FOUR ? D / 32 : D / 8;
+    constexpr int kVRows = 64 / kVLanes;
+    constexpr int kVLoads = (kKeyTile + kVRows - 1) / kVRows;
+    const int v_row = lane / kVLanes;
+    const int v_part = lane % kVLanes;
+    uint4 k_raw[2][FOUR ? 1 : kChunks], v_raw[kVLoads];
+    unsigned k_byte[2], v_byte[kVLoads];
+    auto fetch_k = [&](const Tile& t) {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+        {
+            if (FOUR)
+            {
+                const unsigned char* const at = c.k + t.base[b] * (D / 2) + r * (D / 2) + g * (D / 8);
+                if (D == 128)
+                    k_raw[b][0] = *reinterpret_cast<const uint4*>(at);
+                else
+                {
+                    const uint2 w = *reinterpret_cast<const uint2*>(at);
+                    k_raw[b][0] = make_uint4(w.x, w.y, 0, 0);
+                }
+                k_byte[b] = c.k_scale[t.base[b] * (D / kKvGroup) + r * (D / kKvGroup) + g * D / 4 / kKvGroup];
+            }
+            else
+            {
+                const unsigned char* const at = c.k + t.base[b] * (D * 2) + r * (D * 2) + g * 16;
+#pragma unroll
+                for (int j = 0; j < kChunks; j++)
+                    k_raw[b][j] = *reinterpret_cast<const uint4*>(at + 64 * j);
+            }
+        }
+    };
+    auto fetch_v = [&](const Tile& t) {
+#pragma unroll
+        for (int j = 0; j < kVLoads; j++)
+        {
+            const int local = j * kVRows + v_row;
+            const size_t base = kVRows > 16 ? (local & 16 ? t.base[1] : t.base[0]) : t.base[j * kVRows / 16];
+            if (FOUR)
+            {
+                const unsigned char* const at = c.v + base * (D / 2) + (local & 15) * (D / 2) + v_part * 16;
+                v_raw[j] = *reinterpret_cast<const uint4*>(at);
+                v_byte[j] = c.v_scale[base * (D / kKvGroup) + (local & 15) * (D / kKvGroup) + v_part];
+            }
+            else
+                v_raw[j] = *reinterpret_cast<const uint4*>(c.v + base * (D * 2) + (local & 15) * (D * 2) + v_part * 16);
+        }
+    };
 
     f32x4 o[kBlocks];
 #pragma unroll
@@ -167,116 +290,114 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
         o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
     float row_max = -INFINITY;
     float row_sum = 0.f;
-    unsigned bad = 0;
-
-    const int* const table = c.table + static_cast<long long>(seq) * c.table_stride;
-    const int slot_mask = (1 << c.page_shift) - 1;
     unsigned char* const v_lds = lds[wave];
 
-    for (int i = kv_part(count, split, p.splits) + wave; i < part_end; i += kWaves)
+    int i = split * part_tiles + wave;
+    Tile now{}, next{};
+    if (i < part_end)
     {
-        const int key0 = (i < tiles.sinks ? i : tiles.begin + i - tiles.sinks) << kKeyShift;
-        // Pages of the two blocks of 16 keys (a page holds whole blocks).
-        size_t base[2];
-        bool there[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-        {
-            const int key = key0 + 16 * b;
-            const bool in = key < span_last.end;
-            const int page = table[(in ? key : key0) >> c.page_shift];
-            const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
-            there[b] = in && ok;
-            if (!ok)
-                bad = AWA_KV_BAD_PAGE;
-            base[b] = (((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) + (key & slot_mask);
-        }
-
-        // K rows: lane r of block b holds key 16 b + r.
-        bf16x8 k[2][kChunks];
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int j = 0; j < kChunks; j++)
-            {
-                const size_t at = base[b] + r;
-                if (FOUR)
-                {
-                    const unsigned w = *reinterpret_cast<const unsigned*>(c.k + at * (D / 2) + 16 * j + 4 * g);
-                    const float unit = four_unit(c.k_scale[at * (D / kKvGroup) + j]);
-                    float v[8];
-                    four_values(w, unit, v);
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        k[b][j][e] = static_cast<__bf16>(v[e]);
-                }
-                else
-                    k[b][j] = *reinterpret_cast<const bf16x8*>(c.k + (at * D + 32 * j + 8 * g) * 2);
-            }
-
-        // V rows into LDS; keys that no row of the tile sees as zeros.
-        constexpr int kRowLanes = D / 8;
-        constexpr int kRowsPass = 64 / kRowLanes;
-        bool finite = true;
-#pragma unroll
-        for (int j = 0; j < kKeyTile / kRowsPass; j++)
-        {
-            const int local = j * kRowsPass + lane / kRowLanes;
-            const int chunk = lane % kRowLanes;
-            const int key = key0 + local;
-            const int b = local >> 4;
-            const size_t at = (b ? base[1] : base[0]) + (local & 15);
-            const bool seen = (b ? there[1] : there[0]) && key < span_last.end &&
-                              (key >= span_first.begin || key < span_last.sinks);
-            uint4 w;
-            if (FOUR)
-            {
-                const unsigned codes = *reinterpret_cast<const unsigned*>(c.v + at * (D / 2) + 4 * chunk);
-                const float unit = four_unit(c.v_scale[at * (D / kKvGroup) + chunk / 4]);
-                float v[8];
-                four_values(codes, unit, v);
-                w = make_uint4(cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]), cvt_pk_bf16(v[4], v[5]),
-                               cvt_pk_bf16(v[6], v[7]));
-            }
-            else
-                w = *reinterpret_cast<const uint4*>(c.v + (at * D + 8 * chunk) * 2);
-            if (!seen)
-                w = make_uint4(0, 0, 0, 0);
-            const unsigned words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                finite = finite && (words[e] & 0x7f80u) != 0x7f80u && (words[e] & 0x7f800000u) != 0x7f800000u;
-            *reinterpret_cast<uint4*>(v_lds + (local * kPitch + 8 * chunk) * 2) = w;
-        }
-
+        now = look_up(i);
+        fetch_k(now);
+        fetch_v(now);
+        next = look_up(min(i + kWaves, part_end - 1));
+    }
+#pragma unroll 1
+    for (; i < part_end; i += kWaves)
+    {
+        const int key0 = now.key0;
+        // Whether every row of the tile sees all its keys.
+        const bool whole = now.there == 3u &&
+                           ((key0 >= span_last.begin && key0 + kKeyTile <= span_first.end) ||
+                            key0 + kKeyTile <= span_first.sinks);
         f32x4 acc[2];
 #pragma unroll
         for (int b = 0; b < 2; b++)
         {
+            const float unit = FOUR ? four_unit(k_byte[b]) : 0.f;
             acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < kChunks; j++)
+            {
+                bf16x8 k;
+                if (FOUR)
+                {
+                    const unsigned words[4] = {k_raw[b][0].x, k_raw[b][0].y, k_raw[b][0].z, k_raw[b][0].w};
+                    k = __builtin_bit_cast(bf16x8, four_bf16(words[j], unit));
+                }
+                else
+                    k = __builtin_bit_cast(bf16x8, k_raw[b][j]);
 #pragma unroll
                 for (int e = kPieces - 1; e >= 0; e--)
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][j], q[j][e], acc[b], 0, 0, 0);
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[j][e], acc[b], 0, 0, 0);
+            }
         }
+        // (Behind the last tile the last is fetched again.)
+        fetch_k(next);
+
+        // V into LDS; of tiles that some row sees in part, keys that no row sees
+        // as zeros.
+        bool finite = true;
+#pragma unroll
+        for (int j = 0; j < kVLoads; j++)
+        {
+            const int local = j * kVRows + v_row;
+            uint4 w[FOUR ? 4 : 1];
+            if (FOUR)
+            {
+                const float unit = four_unit(v_byte[j]);
+                const unsigned words[4] = {v_raw[j].x, v_raw[j].y, v_raw[j].z, v_raw[j].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    w[e] = four_bf16(words[e], unit);
+            }
+            else
+                w[0] = v_raw[j];
+            if (!whole)
+            {
+                const int key = key0 + local;
+                const bool seen = ((now.there >> (local >> 4)) & 1u) && key < span_last.end &&
+                                  (key >= span_first.begin || key < span_last.sinks);
+#pragma unroll
+                for (int e = 0; e < (FOUR ? 4 : 1); e++)
+                {
+                    w[e] = seen ? w[e] : make_uint4(0, 0, 0, 0);
+                    finite = finite && finite8(w[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < (FOUR ? 4 : 1); e++)
+                *reinterpret_cast<uint4*>(v_lds + local * kPitch * 2 + v_part * (FOUR ? 64 : 16) + e * 16) = w[e];
+        }
+        const unsigned there = now.there;
+        now = next;
+        fetch_v(now);
+        next = look_up(min(i + 2 * kWaves, part_end - 1));
 
         float x[8];
         float top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 8; e++)
+            x[e] = acc[e >> 2][e & 3] * p.scale_log2;
+        if (!whole)
         {
-            const int key = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
-            const bool seen = there[e >> 2] && key < span.end && (key >= span.begin || key < span.sinks);
-            x[e] = seen ? acc[e >> 2][e & 3] * p.scale_log2 : -INFINITY;
-            top = fmaxf(top, x[e]);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+            {
+                const int key = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
+                const bool seen = ((there >> (e >> 2)) & 1u) && key < span.end && (key >= span.begin || key < span.sinks);
+                x[e] = seen ? x[e] : -INFINITY;
+            }
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            top = fmaxf(top, x[e]);
         top = max_xor32(max_xor16(top));
         if (__any(top > row_max))
         {
-            const float next = fmaxf(row_max, top);
-            const float alpha = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - next);
-            row_max = next;
+            const float m = fmaxf(row_max, top);
+            // (Before the first weight there is nothing but what is not finite.)
+            const float alpha = row_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
+            row_max = m;
             row_sum *= alpha;
 #pragma unroll
             for (int b = 0; b < kBlocks; b++)
@@ -294,52 +415,46 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
         for (int e = 0; e < 8; e++)
             row_sum += F32 ? x[e] : static_cast<float>(w[0][e]);
 
-        // The wave's LDS writes before its transposed reads.
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
-        if (__all(finite))
+        // A NaN or an infinity among the values: its product with the zero weight
+        // of a row that does not see it would be NaN. Those values are added to
+        // the rows that see them (weights are positive), and left out below.
+        if (!__all(finite))
         {
-#pragma unroll
-            for (int b = 0; b < kBlocks; b++)
-            {
-                const unsigned char* const at = v_lds + ((4 * g + (r >> 2)) * kPitch + 16 * b + 4 * (r & 3)) * 2;
-                const i16x4 lohi[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at)),
-                                       __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 16 * kPitch * 2))};
-                const bf16x8 a = __builtin_bit_cast(bf16x8, lohi);
-#pragma unroll
-                for (int e = kPieces - 1; e >= 0; e--)
-                    o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[e], o[b], 0, 0, 0);
-            }
-        }
-        else
-        {
-            // A NaN or an infinity among the values: a product with the zero
-            // weight of a row that does not see it would be NaN, so those rows
-            // are left out key by key.
 #pragma unroll 1
             for (int key = 0; key < kKeyTile; key++)
             {
-                const int owner = (key & 15) >> 2;
-                float weight = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    weight = e == (key >> 4) * 4 + (key & 3) ? (F32 ? x[e] : static_cast<float>(w[0][e])) : weight;
-                weight = __shfl(weight, owner * 16 + r, 64);
-                const int k_at = key0 + key;
-                const bool seen =
-                    there[key >> 4] && k_at < span.end && (k_at >= span.begin || k_at < span.sinks);
+                const int k = key0 + key;
+                const bool sees =
+                    ((there >> (key >> 4)) & 1u) && k < span.end && (k >= span.begin || k < span.sinks);
 #pragma unroll
                 for (int b = 0; b < kBlocks; b++)
+                {
+                    const uint2 v4 =
+                        *reinterpret_cast<const uint2*>(v_lds + key * kPitch * 2 + (16 * b + 4 * g) * 2);
+                    const float value[4] = {bf16_lo(v4.x), bf16_hi(v4.x), bf16_lo(v4.y), bf16_hi(v4.y)};
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                    {
-                        const uint16_t bits =
-                            *reinterpret_cast<const uint16_t*>(v_lds + (key * kPitch + 16 * b + 4 * g + e) * 2);
-                        const float value = __uint_as_float(static_cast<unsigned>(bits) << 16);
-                        if (seen)
-                            o[b][e] = fmaf(weight, value, o[b][e]);
-                    }
+                        o[b][e] += sees && !(fabsf(value[e]) < INFINITY) ? value[e] : 0.f;
+                }
             }
+            for (int j = lane; j < kKeyTile * (D / 8); j += 64)
+            {
+                uint4* const at = reinterpret_cast<uint4*>(v_lds + j / (D / 8) * kPitch * 2 + j % (D / 8) * 16);
+                *at = only_finite8(*at);
+            }
+        }
+        // (A wave's LDS operations are done in their order.)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+        {
+            const unsigned char* const at = v_lds + ((4 * g + (r >> 2)) * kPitch + 16 * b + 4 * (r & 3)) * 2;
+            const i16x4 lohi[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at)),
+                                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 16 * kPitch * 2))};
+            const bf16x8 a = __builtin_bit_cast(bf16x8, lohi);
+#pragma unroll
+            for (int e = kPieces - 1; e >= 0; e--)
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[e], o[b], 0, 0, 0);
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -348,7 +463,6 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
 
     // Join the waves: each lane group holds a part of its row's sum.
     row_sum = sum_xor32(sum_xor16(row_sum));
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     float* const mine = reinterpret_cast<float*>(v_lds);
 #pragma unroll
     for (int b = 0; b < kBlocks; b++)
@@ -377,7 +491,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
 #pragma unroll
     for (int i = 0; i < kWaves; i++)
     {
-        const float weight = __builtin_amdgcn_exp2f(stats[i][out_row][0] - from);
+        // (A wave that saw nothing has zeros, or values that are not finite.)
+        const float weight = stats[i][out_row][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(stats[i][out_row][0] - from);
         sum += weight * stats[i][out_row][1];
         const float* const part = reinterpret_cast<const float*>(lds[i]) + out_row * D + f0;
 #pragma unroll
@@ -408,19 +523,14 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + t * p.out.stride +
                                (static_cast<long long>(out_head) * D + f0) * kElem;
 #pragma unroll
-    for (int e = 0; e < kPer; e += 4)
+    for (int e = 0; e < kPer; e++)
     {
         if (F32)
-            store4(reinterpret_cast<float*>(dst) + e, v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv);
+            reinterpret_cast<float*>(dst)[e] = v[e] * inv;
         else
-            store4(reinterpret_cast<uint16_t*>(dst) + e, v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv);
+            reinterpret_cast<__bf16*>(dst)[e] = static_cast<__bf16>(v[e] * inv);
     }
 }
-
-typedef __attribute__((address_space(3))) char lds_char;
-// (Scalar loads: a vector load of a page would wait for the loads to LDS before
-// it.)
-typedef const __attribute__((address_space(4))) int constant_int;
 
 // 16 bytes a lane from base + offset to the 1 KB of LDS at `lds` (lane order);
 // the kernel waits for it itself. It has no output register.
@@ -428,37 +538,6 @@ __device__ __forceinline__ void load_to_lds(const unsigned char* base, uint32_t 
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base)
                  : "memory", "m0");
-}
-
-// Whether eight bf16 values are finite, and the finite ones of them (else 0).
-__device__ __forceinline__ bool finite8(const uint4& v)
-{
-    const unsigned words[4] = {v.x, v.y, v.z, v.w};
-    unsigned most = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        most = max(most, max(words[e] & 0x7fffu, (words[e] >> 16) & 0x7fffu));
-    return most < 0x7f80u;
-}
-
-__device__ __forceinline__ uint4 only_finite8(const uint4& v)
-{
-    unsigned words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-    {
-        words[e] = (words[e] & 0x7f80u) == 0x7f80u ? words[e] & 0xffff0000u : words[e];
-        words[e] = (words[e] & 0x7f800000u) == 0x7f800000u ? words[e] & 0xffffu : words[e];
-    }
-    return make_uint4(words[0], words[1], words[2], words[3]);
-}
-
-// A value that is the same in all lanes, in scalar registers.
-__device__ __forceinline__ size_t uniform(size_t x)
-{
-    const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
-    const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
-    return static_cast<size_t>(hi) << 32 | lo;
 }
 
 // Workgroups go to the XCDs in turn; each has its own L2. Of every eight units
@@ -530,7 +609,7 @@ __device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
 // are, in that order, what the lane holds of the PV product's operand P^T, and
 // V^T is read in the same key order.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal)
+__global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal, int part_tiles)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kRows = kTileRows;
@@ -616,8 +695,11 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     }
 
     const KvTiles tiles = kv_tiles(first, last, kTileShift);
-    const int t_begin = kv_part(tiles.sinks + tiles.rest, split, p.splits);
-    const int t_end = kv_part(tiles.sinks + tiles.rest, split + 1, p.splits);
+    const int t_count = tiles.sinks + tiles.rest;
+    if (split * part_tiles >= t_count && split > 0)
+        return;
+    const int t_begin = split * part_tiles;
+    const int t_end = split + 1 == p.splits ? t_count : min(t_count, t_begin + part_tiles);
 
     // A wave loads half a 16-key block of every tile.
     constexpr int kLoadRows = kKeys / 4;
@@ -957,9 +1039,11 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
 }
 
 // Joins the parts of a row: M = max m_i, out = sum 2^(m_i - M) o_i / sum
-// 2^(m_i - M) l_i, in the parts' order. One wave a row and query head.
+// 2^(m_i - M) l_i, in the parts' order. One wave a row and query head; `shape`
+// of the row tiles and key tiles whose parts they are.
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p)
+__global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p, int tile_rows, int key_shift,
+                                                       int part_tiles)
 {
     constexpr int kPer = D / 64;
     const KvView& c = p.cache;
@@ -969,11 +1053,19 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
     if (i >= static_cast<long long>(s.rows) * heads)
         return;
     const int lane = threadIdx.x & 63;
+    const int token = static_cast<int>(i / heads);
+    const int head = static_cast<int>(i - static_cast<long long>(token) * heads);
+    const int row0 = (token * p.group + head % p.group) / tile_rows * tile_rows;
+    const int last = min(row0 + tile_rows, s.rows * p.group) - 1;
+    const int slot0 = s.length - s.rows;
+    const KvTiles tiles = kv_tiles(kv_span(p.mask, slot0 + row0 / p.group, s.length),
+                                   kv_span(p.mask, slot0 + last / p.group, s.length), key_shift);
+    const int parts = min(p.splits, max(1, (tiles.sinks + tiles.rest + part_tiles - 1) / part_tiles));
     const size_t all = static_cast<size_t>(c.total_rows) * heads;
     const size_t at = static_cast<size_t>(s.first) * heads + i;
     const float* const stats = p.partial + p.splits * all * D;
     float m = -INFINITY;
-    for (int j = 0; j < p.splits; j++)
+    for (int j = 0; j < parts; j++)
         m = fmaxf(m, stats[(j * all + at) * 2]);
     const float from = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
@@ -981,9 +1073,10 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
 #pragma unroll
     for (int e = 0; e < kPer; e++)
         v[e] = 0.f;
-    for (int j = 0; j < p.splits; j++)
+    for (int j = 0; j < parts; j++)
     {
-        const float weight = __builtin_amdgcn_exp2f(stats[(j * all + at) * 2] - from);
+        const float top = stats[(j * all + at) * 2];
+        const float weight = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - from);
         sum += weight * stats[(j * all + at) * 2 + 1];
         const float* const part = p.partial + (j * all + at) * D + lane * kPer;
 #pragma unroll
@@ -991,9 +1084,8 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
             v[e] = fmaf(weight, part[e], v[e]);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const long long token = i / heads;
     unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + (s.first + token) * p.out.stride +
-                               (i - token * heads) * D * (F32 ? 4 : 2);
+                               static_cast<long long>(head) * D * (F32 ? 4 : 2);
 #pragma unroll
     for (int e = 0; e < kPer; e++)
     {
@@ -1004,61 +1096,48 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
     }
 }
 
-// Row tiles: of 16 where no sequence has more than 32 rows a key/value head,
-// else of 128.
-struct Shape
-{
-    bool few;
-    int rows; // of a tile
-    int tiles;
-};
-
-Shape shape_of(const KvView& c, int group)
-{
-    const long long rows = static_cast<long long>(c.max_rows) * group;
-    Shape s;
-    s.few = rows <= 32;
-    s.rows = s.few ? kRowTile : kTileRows;
-    s.tiles = static_cast<int>((rows + s.rows - 1) / s.rows);
-    return s;
-}
-
-template <int D, bool F32, bool FOUR>
-hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
-{
-    const Shape s = shape_of(p.cache, p.group);
-    if (s.few)
-        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>),
-                           dim3(s.tiles * p.cache.heads * p.splits, p.cache.sequences), dim3(kWaves * 64), 0, stream, p,
-                           s.tiles);
-    else
-    {
-        const TileDeal d = tile_deal(p.cache.heads * p.cache.sequences, s.tiles * p.splits);
-        const dim3 grid(8u * d.period * d.periods);
-        hipLaunchKernelGGL((kv_tile_kernel<D, F32, FOUR>), grid, dim3(256), 0, stream, p, d);
-    }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1)
-        return e;
-    hipLaunchKernelGGL((kv_merge_kernel<D, F32>),
-                       dim3((p.cache.max_rows * p.cache.heads * p.group + 3) / 4, p.cache.sequences), dim3(256), 0,
-                       stream, p);
-    return hipGetLastError();
-}
-
 } // namespace
 
-int kv_attention_splits(const KvView& c, int group, const KvMaskRule& mask, int max_length)
+KvDeal kv_attention_deal(const KvView& c, int group, const KvMaskRule& mask, int max_length)
 {
-    const Shape s = shape_of(c, group);
-    // Keys that a row tile may see, and the workgroups without splitting.
+    const long long rows = static_cast<long long>(c.max_rows) * group;
+    KvDeal d;
+    d.few = rows <= 2 * kRowTile;
+    d.tile_rows = d.few ? kRowTile : kTileRows;
+    d.tiles = static_cast<int>((rows + d.tile_rows - 1) / d.tile_rows);
+    d.key_shift = d.few ? kKeyShift : kTileShift;
+    // Key tiles that a row tile may see, and the workgroups if none is split.
     long long keys = max_length;
     if (mask.window > 0)
         keys = std::min(keys, static_cast<long long>(mask.window) + mask.sinks + mask.block +
-                                  std::min(c.max_rows, s.rows / group + 1));
-    const long long blocks = static_cast<long long>(s.tiles) * c.heads * c.sequences;
-    const long long most = std::max(1ll, keys / 256);
-    return static_cast<int>(std::min({most, std::max(1ll, (s.few ? 2048 : 512) / blocks), 64ll}));
+                                  std::min(c.max_rows, d.tile_rows / group + 1));
+    const long long count = (keys >> d.key_shift) + 2;
+    const long long blocks = static_cast<long long>(d.tiles) * c.heads * c.sequences;
+    d.splits = 1;
+    if (d.few)
+    {
+        // The split with the least time, in key tiles of a workgroup: rounds of
+        // workgroups (768 fit the device), each with its start and its part, and
+        // the join.
+        long long best = 0;
+        for (int n = 1; n <= 64 && n <= count; n++)
+        {
+            const long long part = (count + n - 1) / n;
+            if (n > 1 && part < kWaves)
+                break;
+            const long long time = (blocks * n + 767) / 768 * (part + 8) + (n > 1 ? 16 + n / 4 : 0);
+            if (n == 1 || time < best)
+            {
+                best = time;
+                d.splits = n;
+            }
+        }
+    }
+    else if (blocks < 192)
+        // Too few to fill the device: two a CU, with at least eight key tiles.
+        d.splits = static_cast<int>(std::max(1ll, std::min({(511 + blocks) / blocks, count / 8, 64ll})));
+    d.part_tiles = static_cast<int>((count + d.splits - 1) / d.splits);
+    return d;
 }
 
 size_t kv_attention_partial_bytes(const KvView& c, int group, int head_dim, int splits)
@@ -1067,13 +1146,41 @@ size_t kv_attention_partial_bytes(const KvView& c, int group, int head_dim, int 
                        : static_cast<size_t>(c.total_rows) * c.heads * group * splits * (head_dim + 2) * sizeof(float);
 }
 
-hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream)
+namespace
+{
+
+template <int D, bool F32, bool FOUR>
+hipError_t launch(const KvAttentionLaunch& p, const KvDeal& d, hipStream_t stream)
+{
+    if (d.few)
+    {
+        const dim3 grid(d.tiles * p.cache.heads * d.splits, p.cache.sequences);
+        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p, d.tiles, d.part_tiles);
+    }
+    else
+    {
+        const TileDeal t = tile_deal(p.cache.heads * p.cache.sequences, d.tiles * d.splits);
+        hipLaunchKernelGGL((kv_tile_kernel<D, F32, FOUR>), dim3(8u * t.period * t.periods), dim3(256), 0, stream, p, t,
+                           d.part_tiles);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || d.splits == 1)
+        return e;
+    hipLaunchKernelGGL((kv_merge_kernel<D, F32>),
+                       dim3((p.cache.max_rows * p.cache.heads * p.group + 3) / 4, p.cache.sequences), dim3(256), 0,
+                       stream, p, d.tile_rows, d.key_shift, d.part_tiles);
+    return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t launch_kv_attention(const KvAttentionLaunch& p, const KvDeal& d, hipStream_t stream)
 {
     if (p.head_dim == 128)
-        return p.four ? (p.f32 ? launch<128, true, true>(p, stream) : launch<128, false, true>(p, stream))
-                      : (p.f32 ? launch<128, true, false>(p, stream) : launch<128, false, false>(p, stream));
-    return p.four ? (p.f32 ? launch<64, true, true>(p, stream) : launch<64, false, true>(p, stream))
-                  : (p.f32 ? launch<64, true, false>(p, stream) : launch<64, false, false>(p, stream));
+        return p.four ? (p.f32 ? launch<128, true, true>(p, d, stream) : launch<128, false, true>(p, d, stream))
+                      : (p.f32 ? launch<128, true, false>(p, d, stream) : launch<128, false, false>(p, d, stream));
+    return p.four ? (p.f32 ? launch<64, true, true>(p, d, stream) : launch<64, false, true>(p, d, stream))
+                  : (p.f32 ? launch<64, true, false>(p, d, stream) : launch<64, false, false>(p, d, stream));
 }
 
 } // namespace awa

@@ -111,12 +111,6 @@ __host__ __device__ inline KvTiles kv_tiles(const KvSpan& first, const KvSpan& l
     return t;
 }
 
-// Part i of n of `tiles` tiles: [first, end).
-__host__ __device__ inline int kv_part(int tiles, int i, int n)
-{
-    return static_cast<int>(static_cast<long long>(tiles) * i / n);
-}
-
 // Rotation of the first rope_dim features of a row.
 struct KvRope
 {
@@ -170,9 +164,20 @@ struct KvAttentionLaunch
     float* partial;
 };
 
-// Parts that the work is dealt to, and the bytes of its partial rows.
-int kv_attention_splits(const KvView& cache, int group, const KvMaskRule& mask, int max_length);
+// How the work is dealt out: row tiles of one kernel or the other, and of each
+// the key tiles in parts of part_tiles, at most `splits`.
+struct KvDeal
+{
+    bool few; // rows: tiles of 16
+    int tile_rows, tiles; // rows of a row tile, row tiles of the longest sequence
+    int key_shift;
+    int splits, part_tiles;
+};
+
+// max_length: a bound of the lengths (the last part takes what longer ones have
+// beyond it).
+KvDeal kv_attention_deal(const KvView& cache, int group, const KvMaskRule& mask, int max_length);
 size_t kv_attention_partial_bytes(const KvView& cache, int group, int head_dim, int splits);
-hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream);
+hipError_t launch_kv_attention(const KvAttentionLaunch& p, const KvDeal& deal, hipStream_t stream);
 
 } // namespace awa

@@ -594,12 +594,12 @@ def test_captured_step_follows_the_lengths(gpu):
     """An append, an attention and a read in a graph, replayed while lengths
     and inputs change, with the same calls made eagerly between the replays."""
     rng = np.random.default_rng(31)
-    cache = M.Cache("4bit", [1000, 2000], 2, 128, 16)
+    cache = M.Cache("4bit", [6000, 9000], 2, 128, 16)
     cache.lengths[:] = [400, 900]
     desc = cache.upload()
     shapes = {"q": 4, "k": 2, "v": 2, "qo": 4, "out": 4, "kr": 2, "vr": 2}
     t = {n: M.Rows(np.zeros((2, h, 128)), "bf16") for n, h in shapes.items()}
-    rows, mask, rope = A.KvRows(1), A.KvMask(640, 4, 1), A.Rope(128, halves=True)
+    rows, mask, rope = A.KvRows(1), A.KvMask(0, 4, 1), A.Rope(128, halves=True)
     n = A.kv_attention_workspace(desc, rows, t["q"].blob, mask)
     assert n > 0
     ws = A.DeviceBuffer(n)
@@ -624,7 +624,7 @@ def test_captured_step_follows_the_lengths(gpu):
     for i in range(4):
         for m in ("q", "k", "v"):
             t[m].buf.upload(A.f32_to_bf16_bits(rng.standard_normal(t[m].shape).astype(np.float32)))
-        cache.set(lengths=[401 + 130 * i, 901 + 300 * i])
+        cache.set(lengths=[401 + 1300 * i, 901 + 2600 * i])
         assert rt.hipGraphLaunch(run, s) == 0
         replayed = results()
         pools = cache.download()
@@ -640,7 +640,7 @@ def test_captured_step_follows_the_lengths(gpu):
         for j in range(2):
             k, _ = cache.rows("k", j)
             v, _ = cache.rows("v", j)
-            want, bound = M.attention(replayed["qo"][j:j + 1], k, v, int(cache.lengths[j]), 640, 4, 1, 128 ** -0.5,
+            want, bound = M.attention(replayed["qo"][j:j + 1], k, v, int(cache.lengths[j]), 0, 4, 1, 128 ** -0.5,
                                       "bf16")
             assert (np.abs(replayed["out"][j:j + 1] - want) <= bound).all()
     assert rt.hipGraphExecDestroy(run) == 0 and rt.hipGraphDestroy(graph) == 0
