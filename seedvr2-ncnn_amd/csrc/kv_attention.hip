@@ -117,6 +117,20 @@ __device__ __forceinline__ uint4 only_finite8(const uint4& v)
     return make_uint4(words[0], words[1], words[2], words[3]);
 }
 
+// A part's row and its (maximum, sum): all rows of part 0, of part 1, ..., then
+// the pairs.
+__device__ __forceinline__ float* part_row(const KvAttentionLaunch& p, int dim, int part, size_t row, int head)
+{
+    const size_t all = static_cast<size_t>(p.cache.total_rows) * p.heads.d;
+    return p.partial + (part * all + row * p.heads.d + head) * dim;
+}
+
+__device__ __forceinline__ float* part_stats(const KvAttentionLaunch& p, int dim, int part, size_t row, int head)
+{
+    const size_t all = static_cast<size_t>(p.cache.total_rows) * p.heads.d;
+    return p.partial + p.splits * all * dim + (part * all + row * p.heads.d + head) * 2;
+}
+
 // One row tile of 16 rows, one part of its keys: each wave takes every fourth
 // key tile (32 keys) by itself, with K from memory straight into the MFMA
 // operand registers and V through the wave's own LDS, from which it is read
@@ -131,7 +145,7 @@ __device__ __forceinline__ uint4 only_finite8(const uint4& v)
 // matter as long as both operands agree: of 4-bit rows a lane has a quarter,
 // one load and one scale.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p, int row_tiles, int part_tiles)
+__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p, int two_tiles, int part_tiles)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kChunks = D / 32;
@@ -144,40 +158,46 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     __shared__ float stats[kWaves][kRowTile][2];
 
     const KvView& c = p.cache;
-    const int seq = blockIdx.y;
+    const int seq = blockIdx.z;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15;
     const int g = lane >> 4;
-    int block = blockIdx.x;
-    const int split = block % p.splits;
-    block /= p.splits;
-    const int tile = block % row_tiles;
-    const int head = block / row_tiles;
+    const int head = blockIdx.y;
+    const int tile = blockIdx.x & two_tiles; // one or two row tiles
+    const int split = blockIdx.x >> two_tiles;
 
     const KvSequence s = kv_sequence(c, seq);
     if (s.bad && c.status && threadIdx.x == 0)
         atomicOr(c.status, static_cast<int>(s.bad));
-    const int rows = s.rows * p.group;
+    const int rows = s.rows * p.group.d;
     const int row0 = tile * kRowTile;
     if (row0 >= rows)
         return;
     const int last = min(row0 + kRowTile, rows) - 1;
     const int slot0 = s.length - s.rows;
-    const KvSpan span_first = kv_span(p.mask, slot0 + row0 / p.group, s.length);
-    const KvSpan span_last = kv_span(p.mask, slot0 + last / p.group, s.length);
+    const KvSpan span_first = kv_span(p.mask, slot0 + kv_divide(row0, p.group), s.length);
+    const KvSpan span_last = kv_span(p.mask, slot0 + kv_divide(last, p.group), s.length);
     const KvTiles tiles = kv_tiles(span_first, span_last, kKeyShift);
     const int count = tiles.sinks + tiles.rest;
-    // (The first part joins in for rows that see nothing.)
-    if (split * part_tiles >= count && split > 0)
+    if (split * part_tiles >= count && p.splits > 1)
+    {
+        // No keys: the join leaves this part out.
+        const int i = row0 + threadIdx.x;
+        if (threadIdx.x < kRowTile && i <= last)
+        {
+            const int t = kv_divide(i, p.group);
+            part_stats(p, D, split, s.first + t, head * p.group.d + i - t * p.group.d)[0] = -INFINITY;
+        }
         return;
+    }
     // (The last one takes all that is left: lengths may pass their bound.)
     const int part_end = split + 1 == p.splits ? count : min(count, (split + 1) * part_tiles);
 
     // This lane's row (rows past the end repeat the last; they are not stored).
     const int row = min(row0 + r, last);
-    const int token = row / p.group;
-    const int q_head = head * p.group + row - token * p.group;
+    const int token = kv_divide(row, p.group);
+    const int q_head = head * p.group.d + row - token * p.group.d;
     const KvSpan span = kv_span(p.mask, slot0 + token, s.length);
     bf16x8 q[kChunks][kPieces];
     {
@@ -491,32 +511,26 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
 #pragma unroll
     for (int i = 0; i < kWaves; i++)
     {
-        // (A wave that saw nothing has zeros, or values that are not finite.)
-        const float weight = stats[i][out_row][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(stats[i][out_row][0] - from);
+        if (stats[i][out_row][0] == -INFINITY)
+            continue;
+        const float weight = __builtin_amdgcn_exp2f(stats[i][out_row][0] - from);
         sum += weight * stats[i][out_row][1];
         const float* const part = reinterpret_cast<const float*>(lds[i]) + out_row * D + f0;
 #pragma unroll
         for (int e = 0; e < kPer; e++)
             v[e] = fmaf(weight, part[e], v[e]);
     }
-    const int out_token = (row0 + out_row) / p.group;
-    const int out_head = head * p.group + (row0 + out_row) - out_token * p.group;
+    const int out_token = kv_divide(row0 + out_row, p.group);
+    const int out_head = head * p.group.d + row0 + out_row - out_token * p.group.d;
     const long long t = s.first + out_token;
     if (p.splits > 1)
     {
-        const size_t heads = static_cast<size_t>(c.heads) * p.group;
-        const size_t all = static_cast<size_t>(c.total_rows) * heads;
-        const size_t at = split * all + t * heads + out_head;
-        float* const dst = p.partial + at * D + f0;
+        float* const dst = part_row(p, D, split, t, out_head) + f0;
 #pragma unroll
         for (int e = 0; e < kPer; e++)
             dst[e] = v[e];
         if (f0 == 0)
-        {
-            float* const st = p.partial + p.splits * all * D + at * 2;
-            st[0] = m;
-            st[1] = sum;
-        }
+            *reinterpret_cast<float2*>(part_stats(p, D, split, t, out_head)) = make_float2(m, sum);
         return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -647,12 +661,12 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     const KvSequence s = kv_sequence(c, seq);
     if (s.bad && c.status && tid == 0)
         atomicOr(c.status, static_cast<int>(s.bad));
-    const int rows = s.rows * p.group;
+    const int rows = s.rows * p.group.d;
     const int row0 = tile * kRows;
     if (row0 >= rows)
         return;
     const int slot0 = s.length - s.rows;
-    auto span_of = [&](int row) { return kv_span(p.mask, slot0 + row / p.group, s.length); };
+    auto span_of = [&](int row) { return kv_span(p.mask, slot0 + kv_divide(row, p.group), s.length); };
     const KvSpan first = span_of(row0);
     const KvSpan last = span_of(min(row0 + kRows, rows) - 1);
 
@@ -662,8 +676,8 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     const KvSpan w_first = span_of(min(wave_row0, rows - 1));
     const KvSpan w_last = span_of(min(wave_row0 + 32, rows) - 1);
     const int row = min(wave_row0 + col, rows - 1);
-    const int token = row / p.group;
-    const int q_head = head * p.group + row - token * p.group;
+    const int token = kv_divide(row, p.group);
+    const int q_head = head * p.group.d + row - token * p.group.d;
     const KvSpan span = kv_span(p.mask, slot0 + token, s.length);
     bf16x8 q[kC][kPieces];
     // (Not zero, whose product with the -inf of a masked score is NaN.)
@@ -696,8 +710,12 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
 
     const KvTiles tiles = kv_tiles(first, last, kTileShift);
     const int t_count = tiles.sinks + tiles.rest;
-    if (split * part_tiles >= t_count && split > 0)
+    if (split * part_tiles >= t_count && p.splits > 1)
+    {
+        if (half == 0 && wave_row0 + col < rows)
+            part_stats(p, D, split, s.first + token, q_head)[0] = -INFINITY;
         return;
+    }
     const int t_begin = split * part_tiles;
     const int t_end = split + 1 == p.splits ? t_count : min(t_count, t_begin + part_tiles);
 
@@ -1017,16 +1035,9 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     const long long at = s.first + token;
     if (p.splits > 1)
     {
-        const size_t heads = static_cast<size_t>(c.heads) * p.group;
-        const size_t all = static_cast<size_t>(c.total_rows) * heads;
-        const size_t i = split * all + at * heads + q_head;
-        store_o(p.partial + i * D, o, 1.f, half);
+        store_o(part_row(p, D, split, at, q_head), o, 1.f, half);
         if (half == 0)
-        {
-            float* const st = p.partial + p.splits * all * D + i * 2;
-            st[0] = row_max;
-            st[1] = sum;
-        }
+            *reinterpret_cast<float2*>(part_stats(p, D, split, at, q_head)) = make_float2(row_max, sum);
         return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -1039,52 +1050,64 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
 }
 
 // Joins the parts of a row: M = max m_i, out = sum 2^(m_i - M) o_i / sum
-// 2^(m_i - M) l_i, in the parts' order. One wave a row and query head; `shape`
-// of the row tiles and key tiles whose parts they are.
+// 2^(m_i - M) l_i, in the parts' order; parts without a key are left out. One
+// wave a row and query head. Bound by latency: all parts' maxima and sums come
+// with one load, their rows with independent ones.
 template <int D, bool F32>
-__global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p, int tile_rows, int key_shift,
-                                                       int part_tiles)
+__global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p)
 {
     constexpr int kPer = D / 64;
+    constexpr int kBatch = 8;
     const KvView& c = p.cache;
     const KvSequence s = kv_sequence(c, blockIdx.y);
-    const int heads = c.heads * p.group;
-    const long long i = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (i >= static_cast<long long>(s.rows) * heads)
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= s.rows * p.heads.d)
         return;
     const int lane = threadIdx.x & 63;
-    const int token = static_cast<int>(i / heads);
-    const int head = static_cast<int>(i - static_cast<long long>(token) * heads);
-    const int row0 = (token * p.group + head % p.group) / tile_rows * tile_rows;
-    const int last = min(row0 + tile_rows, s.rows * p.group) - 1;
-    const int slot0 = s.length - s.rows;
-    const KvTiles tiles = kv_tiles(kv_span(p.mask, slot0 + row0 / p.group, s.length),
-                                   kv_span(p.mask, slot0 + last / p.group, s.length), key_shift);
-    const int parts = min(p.splits, max(1, (tiles.sinks + tiles.rest + part_tiles - 1) / part_tiles));
-    const size_t all = static_cast<size_t>(c.total_rows) * heads;
-    const size_t at = static_cast<size_t>(s.first) * heads + i;
-    const float* const stats = p.partial + p.splits * all * D;
-    float m = -INFINITY;
-    for (int j = 0; j < parts; j++)
-        m = fmaxf(m, stats[(j * all + at) * 2]);
-    const float from = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
+    const int token = kv_divide(i, p.heads);
+    const int head = i - token * p.heads.d;
+    const size_t row = static_cast<size_t>(s.first) + token;
+    const float2 mine = lane < p.splits ? *reinterpret_cast<const float2*>(part_stats(p, D, lane, row, head))
+                                        : make_float2(-INFINITY, 0.f);
+    float m = mine.x;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1)
+        m = fmaxf(m, __shfl_xor(m, off, 64));
+    const bool there = mine.x != -INFINITY;
+    const float weight = there ? __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.f : m)) : 0.f;
+    float sum = there ? weight * mine.y : 0.f;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1)
+        sum += __shfl_xor(sum, off, 64);
+    unsigned long long left = __ballot(there);
     float v[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; e++)
         v[e] = 0.f;
-    for (int j = 0; j < parts; j++)
+    while (left)
     {
-        const float top = stats[(j * all + at) * 2];
-        const float weight = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - from);
-        sum += weight * stats[(j * all + at) * 2 + 1];
-        const float* const part = p.partial + (j * all + at) * D + lane * kPer;
+        float part[kBatch][kPer], by[kBatch];
 #pragma unroll
-        for (int e = 0; e < kPer; e++)
-            v[e] = fmaf(weight, part[e], v[e]);
+        for (int b = 0; b < kBatch; b++)
+        {
+            // (Past the last part: that one again, with no weight.)
+            const int j = __builtin_amdgcn_readfirstlane(left ? __ffsll(left) - 1 : 0);
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j));
+            const float* const src = part_row(p, D, j, row, head) + lane * kPer;
+            by[b] = left ? w : 0.f;
+#pragma unroll
+            for (int e = 0; e < kPer; e++)
+                part[b][e] = left ? src[e] : 0.f;
+            left &= left - 1;
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; b++)
+#pragma unroll
+            for (int e = 0; e < kPer; e++)
+                v[e] = fmaf(by[b], part[b][e], v[e]);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + (s.first + token) * p.out.stride +
+    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + static_cast<long long>(row) * p.out.stride +
                                static_cast<long long>(head) * D * (F32 ? 4 : 2);
 #pragma unroll
     for (int e = 0; e < kPer; e++)
@@ -1098,7 +1121,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
 
 } // namespace
 
-KvDeal kv_attention_deal(const KvView& c, int group, const KvMaskRule& mask, int max_length)
+KvDeal kv_attention_deal(const KvView& c, int group, int head_dim, bool four, const KvMaskRule& mask, int max_length)
 {
     const long long rows = static_cast<long long>(c.max_rows) * group;
     KvDeal d;
@@ -1117,15 +1140,16 @@ KvDeal kv_attention_deal(const KvView& c, int group, const KvMaskRule& mask, int
     if (d.few)
     {
         // The split with the least time, in key tiles of a workgroup: rounds of
-        // workgroups (768 fit the device), each with its start and its part, and
-        // the join.
+        // workgroups (two or three a CU, by their registers), each with its start
+        // and its part, and the join.
+        const long long slots = 256 * (four || head_dim == 64 ? 3 : 2);
         long long best = 0;
         for (int n = 1; n <= 64 && n <= count; n++)
         {
             const long long part = (count + n - 1) / n;
             if (n > 1 && part < kWaves)
                 break;
-            const long long time = (blocks * n + 767) / 768 * (part + 8) + (n > 1 ? 16 + n / 4 : 0);
+            const long long time = (blocks * n + slots - 1) / slots * (part + 8) + (n > 1 ? 16 + n / 4 : 0);
             if (n == 1 || time < best)
             {
                 best = time;
@@ -1154,8 +1178,9 @@ hipError_t launch(const KvAttentionLaunch& p, const KvDeal& d, hipStream_t strea
 {
     if (d.few)
     {
-        const dim3 grid(d.tiles * p.cache.heads * d.splits, p.cache.sequences);
-        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p, d.tiles, d.part_tiles);
+        const dim3 grid(d.tiles * d.splits, p.cache.heads, p.cache.sequences);
+        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p, d.tiles - 1,
+                           d.part_tiles);
     }
     else
     {
@@ -1167,8 +1192,7 @@ hipError_t launch(const KvAttentionLaunch& p, const KvDeal& d, hipStream_t strea
     if (e != hipSuccess || d.splits == 1)
         return e;
     hipLaunchKernelGGL((kv_merge_kernel<D, F32>),
-                       dim3((p.cache.max_rows * p.cache.heads * p.group + 3) / 4, p.cache.sequences), dim3(256), 0,
-                       stream, p, d.tile_rows, d.key_shift, d.part_tiles);
+                       dim3((p.cache.max_rows * p.heads.d + 3) / 4, p.cache.sequences), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

@@ -137,14 +137,16 @@ int attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob
     if (q->h % cache->kv_heads)
         return invalid("query heads must be a multiple of the cache's heads");
     p.head_dim = cache->head_dim;
-    p.group = q->h / cache->kv_heads;
+    const int group = q->h / cache->kv_heads;
+    p.group = awa::kv_divisor(group);
+    p.heads = awa::kv_divisor(q->h);
     p.f32 = q->elemsize == 4;
     p.four = cache->format == AWA_KV_MXFP4;
     const long long slots = static_cast<long long>(cache->table_width) * cache->page_tokens;
     const long long longest = mask->max_length > 0 && mask->max_length < slots ? mask->max_length : slots;
     if (static_cast<long long>(p.cache.max_rows) * q->h >= 1ll << 30)
         return invalid("max_rows times query heads must be below 2^30");
-    d = awa::kv_attention_deal(p.cache, p.group, p.mask, static_cast<int>(longest));
+    d = awa::kv_attention_deal(p.cache, group, p.head_dim, p.four, p.mask, static_cast<int>(longest));
     p.splits = d.splits;
     if (8ll * (static_cast<long long>(cache->sequences) * cache->kv_heads + 8) * (static_cast<long long>(d.tiles) * d.splits + 8) >= 1ll << 34)
         return invalid("too many rows, heads and sequences for one call");
@@ -282,7 +284,7 @@ int awa_kv_attention_workspace(const awa_kv_cache* cache, const awa_kv_rows* row
     awa::KvDeal d{};
     const int rc = attention(cache, rows, q, mask, p, d);
     if (rc == AWA_OK)
-        *bytes = awa::kv_attention_partial_bytes(p.cache, p.group, p.head_dim, p.splits);
+        *bytes = awa::kv_attention_partial_bytes(p.cache, p.group.d, p.head_dim, p.splits);
     return rc;
 }
 
@@ -301,7 +303,7 @@ int awa_kv_attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const a
     if (!std::isfinite(scale))
         return invalid("the scale must be finite");
     p.scale_log2 = scale * 1.44269504088896340736f;
-    const size_t need = awa::kv_attention_partial_bytes(p.cache, p.group, p.head_dim, p.splits);
+    const size_t need = awa::kv_attention_partial_bytes(p.cache, p.group.d, p.head_dim, p.splits);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return invalid("this call needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
     p.partial = static_cast<float*>(workspace);
@@ -314,6 +316,11 @@ int awa_kv_host_sequence(int first, int end, int length, int capacity, int max_r
     const awa::KvSequence s = awa::kv_sequence(first, end, length, capacity, max_rows, total_rows);
     out[0] = s.first, out[1] = s.rows, out[2] = s.length, out[3] = static_cast<int>(s.bad);
     return AWA_OK;
+}
+
+int awa_kv_host_divide(int n, int d)
+{
+    return awa::kv_divide(n, awa::kv_divisor(d));
 }
 
 int awa_kv_host_span(int window, int sinks, int block, int slot, int length, int* out)

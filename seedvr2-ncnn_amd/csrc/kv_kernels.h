@@ -31,6 +31,28 @@ struct KvView
     int max_rows, total_rows;
 };
 
+// floor(n / d) for 0 <= n < 2^30 as a multiplication: with 2^(s - 1) < d <= 2^s
+// and m = floor(2^(30 + s) / d) + 1, m d is above 2^(30 + s) by at most 2^s, so
+// that n m / 2^(30 + s) is above n / d by less than 1 / d.
+struct KvDivisor
+{
+    unsigned m;
+    int shift, d;
+};
+
+__host__ inline KvDivisor kv_divisor(int d)
+{
+    int s = 0;
+    while ((1ll << s) < d)
+        s++;
+    return {static_cast<unsigned>((1ull << (30 + s)) / d + 1), 30 + s, d};
+}
+
+__host__ __device__ inline int kv_divide(int n, const KvDivisor& by)
+{
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * by.m) >> by.shift);
+}
+
 // The new rows of one sequence: packed rows [first, first + rows), at slots
 // [length - rows, length). What does not fit together (bad != 0) has no rows,
 // so that nothing of it is read or written.
@@ -153,7 +175,9 @@ hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t stream);
 struct KvAttentionLaunch
 {
     KvView cache;
-    int head_dim, group; // query heads a key/value head
+    int head_dim;
+    KvDivisor group; // query heads a key/value head
+    KvDivisor heads; // query heads
     bool f32, four;
     KvRowsSource q, out;
     KvMaskRule mask;
@@ -176,7 +200,7 @@ struct KvDeal
 
 // max_length: a bound of the lengths (the last part takes what longer ones have
 // beyond it).
-KvDeal kv_attention_deal(const KvView& cache, int group, const KvMaskRule& mask, int max_length);
+KvDeal kv_attention_deal(const KvView& cache, int group, int head_dim, bool four, const KvMaskRule& mask, int max_length);
 size_t kv_attention_partial_bytes(const KvView& cache, int group, int head_dim, int splits);
 hipError_t launch_kv_attention(const KvAttentionLaunch& p, const KvDeal& deal, hipStream_t stream);
 

@@ -219,3 +219,15 @@ def test_model_of_the_four_bit_rows():
     y = np.abs(x) / unit
     step = np.where(y < 2, 0.5, np.where(y < 4, 1.0, 2.0))
     assert (np.abs(M.decode4(codes, byte) - x) <= step / 2 * unit).all()
+
+
+def test_division_by_a_multiplication():
+    """Every divisor to 200 and large ones, at multiples and beside them, up to 2^30."""
+    rng = np.random.default_rng(1)
+    divide = A.lib().awa_kv_host_divide
+    for d in list(range(1, 201)) + [1 << 10, (1 << 10) + 1, 65535, 65536, 65537, (1 << 29) + 3, (1 << 30) - 1]:
+        top = (1 << 30) - 1
+        q = [0, 1, top // d] + [int(x) for x in rng.integers(0, top // d + 1, 30)]
+        for n in {x for k in q for x in (k * d - 1, k * d, k * d + 1, k * d + d - 1)} | {top, 0}:
+            if 0 <= n <= top:
+                assert divide(n, d) == n // d, (n, d)
