@@ -427,7 +427,7 @@ int awa_dit_stack_block_times(const awa_dit_stack* stack, float* block_ms);
  * (the new rows included) and n new rows, row j has slot L - n + j. So one
  * descriptor serves the append, the attention and the read of a step.
  *
- * Pools, [pages][kv_heads][page_tokens] rows of head_dim features:
+ * Pools, [pages][kv_heads][page_tokens] (less than 2^31) rows of head_dim features:
  *   AWA_KV_BF16: bf16.
  *   AWA_KV_MXFP4: four bits a feature, e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6
  *     and sign), the even feature in a byte's low half; and in k_scale /

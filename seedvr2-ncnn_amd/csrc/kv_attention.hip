@@ -86,14 +86,6 @@ typedef __attribute__((address_space(3))) char lds_char;
 // it.)
 typedef const __attribute__((address_space(4))) int constant_int;
 
-// A value that is the same in all lanes, in scalar registers.
-__device__ __forceinline__ size_t uniform(size_t x)
-{
-    const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
-    const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
-    return static_cast<size_t>(hi) << 32 | lo;
-}
-
 // Whether eight bf16 values are finite, and the finite ones of them (else 0).
 __device__ __forceinline__ bool finite8(const uint4& v)
 {
@@ -227,7 +219,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     const int slot_mask = (1 << c.page_shift) - 1;
     unsigned bad = 0;
     // A key tile: its first key, which of its two 16-key blocks are there, and
-    // their pool rows.
+    // their pool rows (of which there are less than 2^31). (A block behind the
+    // last key has the last key's page; it is masked.)
     struct Tile
     {
         int key0;
@@ -248,8 +241,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
                 t.there |= 1u << b;
             if (!ok)
                 bad = AWA_KV_BAD_PAGE;
-            t.base[b] =
-                uniform((((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) + (key & slot_mask));
+            t.base[b] = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(
+                (((ok ? page : 0) * c.heads + head) << c.page_shift) + (key & slot_mask)));
         }
         return t;
     };
@@ -641,8 +634,6 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     __shared__ __attribute__((aligned(1024))) unsigned char v_lds[2][kTileBytes];
     // The last tile with values that are not finite.
     __shared__ int raw_tile;
-    // Which of a tile's two 16-key blocks have no page; of tile t at t % 4.
-    __shared__ unsigned no_page[4];
 
     const KvView& c = p.cache;
     const int tid = threadIdx.x;
@@ -675,16 +666,26 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     const bool active = wave_row0 < rows;
     const KvSpan w_first = span_of(min(wave_row0, rows - 1));
     const KvSpan w_last = span_of(min(wave_row0 + 32, rows) - 1);
-    const int row = min(wave_row0 + col, rows - 1);
-    const int token = kv_divide(row, p.group);
-    const int q_head = head * p.group.d + row - token * p.group.d;
-    const KvSpan span = kv_span(p.mask, slot0 + token, s.length);
+    // (Worked out again where it is needed: registers are what limits how many
+    // workgroups a CU holds. The lane is hidden from the compiler for that.)
+    struct Row
+    {
+        int token, head;
+    };
+    auto my_row = [&]() {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const int r = min(wave_row0 + (l & 31), rows - 1);
+        const int token = kv_divide(r, p.group);
+        return Row{token, head * p.group.d + r - token * p.group.d};
+    };
     bf16x8 q[kC][kPieces];
     // (Not zero, whose product with the -inf of a masked score is NaN.)
     const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);
     {
-        const unsigned char* src = p.q.data + static_cast<long long>(s.first + token) * p.q.stride +
-                                   static_cast<long long>(q_head) * D * kElem;
+        const Row row = my_row();
+        const unsigned char* src = p.q.data + static_cast<long long>(s.first + row.token) * p.q.stride +
+                                   static_cast<long long>(row.head) * D * kElem;
 #pragma unroll
         for (int i = 0; i < kC; i++)
         {
@@ -712,8 +713,9 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     const int t_count = tiles.sinks + tiles.rest;
     if (split * part_tiles >= t_count && p.splits > 1)
     {
+        const Row row = my_row();
         if (half == 0 && wave_row0 + col < rows)
-            part_stats(p, D, split, s.first + token, q_head)[0] = -INFINITY;
+            part_stats(p, D, split, s.first + row.token, row.head)[0] = -INFINITY;
         return;
     }
     const int t_begin = split * part_tiles;
@@ -724,24 +726,31 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     const int load_row = wave * kLoadRows;
     constant_int* const table = (constant_int*)(c.table + static_cast<long long>(seq) * c.table_stride);
     const int slot_mask = (1 << c.page_shift) - 1;
-    unsigned bad = 0;
     auto tile_key = [&](int t) {
         t = min(t, t_end - 1);
         return (t < tiles.sinks ? t : tiles.begin + t - tiles.sinks) << kTileShift;
     };
-    // (Blocks behind the last key have the last key's page; their rows are
-    // masked.)
-    auto page_of = [&](int key0) { return table[min(key0 + load_row, last.end - 1) >> c.page_shift]; };
-    auto pool_row_of = [&](int t, int key0, int page) {
-        const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
-        if (!ok)
-        {
-            bad = AWA_KV_BAD_PAGE;
-            if (lane == 0)
-                atomicOr(&no_page[t & 3], 1u << (wave >> 1));
-        }
-        return uniform((((ok ? static_cast<size_t>(page) : 0) * c.heads + head) << c.page_shift) +
-                       ((key0 + load_row) & slot_mask));
+    // The pages of a tile's two 16-key blocks, read a tile ahead. (A block behind
+    // the last key has the last key's page; it is masked.)
+    struct Pages
+    {
+        int at[2];
+    };
+    auto pages_of = [&](int key0) {
+        return Pages{{table[min(key0, last.end - 1) >> c.page_shift],
+                      table[min(key0 + 16, last.end - 1) >> c.page_shift]}};
+    };
+    // Which blocks have no page of the pool.
+    auto missing = [&](const Pages& pages) {
+        return static_cast<unsigned>(static_cast<unsigned>(pages.at[0]) >= static_cast<unsigned>(c.pages)) |
+               static_cast<unsigned>(static_cast<unsigned>(pages.at[1]) >= static_cast<unsigned>(c.pages)) << 1;
+    };
+    // The pool row of the wave's first row of the tile (pools have less than 2^31
+    // rows).
+    auto pool_row_of = [&](int key0, const Pages& pages, unsigned none) {
+        const int page = (none >> (wave >> 1)) & 1u ? 0 : wave < 2 ? pages.at[0] : pages.at[1];
+        return static_cast<size_t>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(
+            ((page * c.heads + head) << c.page_shift) + ((key0 + load_row) & slot_mask))));
     };
 
     // Where a 16-byte chunk of a row lies in LDS: chunks are permuted so that
@@ -801,7 +810,9 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
 #pragma unroll
         for (int i = 0; i < 16; i++)
             o[d][i] = 0.f;
-    float row_max = -INFINITY, neg_max = 0.f, row_sum = 0.f;
+    // (Finite, so that no difference is NaN; nothing that is weighed is below.)
+    constexpr float kNoMax = -1.5e38f;
+    float row_max = kNoMax, row_sum = 0.f;
     bf16x8 w[2][kPieces]; // a block's weights
 
     bf16x8 ka[kC], va[2][kDb];
@@ -856,7 +867,7 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
         float y[16];
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            y[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale, neg_max));
+            y[i] = __builtin_amdgcn_exp2f(fmaf(x[i], scale, -row_max));
 #pragma unroll
         for (int j = 0; j < 2; j++)
         {
@@ -888,6 +899,7 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     // does not see them would be NaN). Weights are positive, so what they weigh
     // does not matter.
     auto add_raw = [&](const unsigned char* v, int key0, unsigned none) {
+        const KvSpan span = kv_span(p.mask, slot0 + my_row().token, s.length);
 #pragma unroll 1
         for (int key = 0; key < kKeys; key++)
         {
@@ -912,19 +924,21 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
     auto wait = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // (LDS alone: the loads of the next tile go on.)
     auto wait_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // The first keys of this tile and the next, and the next one's page.
-    int key_now = 0, key_next = 0, page_next = 0;
+    // The first keys of this tile and the next, the next one's pages, and which
+    // blocks of this tile (and of any) have none.
+    int key_now = 0, key_next = 0;
+    Pages pages_next{};
+    unsigned none = 0, bad = 0;
     if (t_begin < t_end)
     {
-        if (tid < 4)
-            no_page[tid] = 0u;
-        if (tid == 4)
+        if (tid == 0)
             raw_tile = -1;
-        __syncthreads();
         key_now = tile_key(t_begin);
         key_next = tile_key(t_begin + 1);
-        const size_t row_now = pool_row_of(t_begin, key_now, page_of(key_now));
-        page_next = page_of(key_next);
+        const Pages pages = pages_of(key_now);
+        pages_next = pages_of(key_next);
+        none = missing(pages);
+        const size_t row_now = pool_row_of(key_now, pages, none);
         if (FOUR)
             load_four(row_now);
         else
@@ -941,21 +955,23 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
         // This tile is there, and all waves are done with the one before.
         // (Behind the last tile the last is loaded again.)
         wait();
-        const size_t row_next = pool_row_of(t + 1, key_next, page_next);
+        const unsigned none_next = missing(pages_next);
+        const size_t row_next = pool_row_of(key_next, pages_next, none_next);
         if (FOUR)
             load_four(row_next);
         else
             load(row_next, 1 - slot);
-        const unsigned none = no_page[t & 3];
-        if (tid == 0)
-            no_page[(t + 2) & 3] = 0u; // tile t - 2's, which nobody needs any more
+        bad |= none;
         const int key_third = tile_key(t + 2);
-        page_next = page_of(key_third);
+        pages_next = pages_of(key_third);
+        bool edge = false;
         // Tiles that some row sees in part. What no row of the workgroup sees
         // becomes zeros, and so do values that are not finite.
         if (none != 0u ||
             !((key_now >= last.begin && key_now + kKeys <= first.end) || key_now + kKeys <= first.sinks))
         {
+            edge = none != 0u || !((key_now >= w_last.begin && key_now + kKeys <= w_first.end) ||
+                                   key_now + kKeys <= w_first.sinks);
             uint4* const v = reinterpret_cast<uint4*>(v_tile);
             constexpr int kMine = kKeys * kRowChunks / kThreads;
             bool fine = true;
@@ -989,9 +1005,9 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
             f32x16 x;
             qk(x);
             float top = top_of(x) * scale;
-            if (none != 0u || !((key_now >= w_last.begin && key_now + kKeys <= w_first.end) ||
-                                key_now + kKeys <= w_first.sinks))
+            if (edge)
             {
+                const KvSpan span = kv_span(p.mask, slot0 + my_row().token, s.length);
                 const int key0 = key_now + 4 * half;
                 const int end = span.end - key0, begin = span.begin - key0, sinks = span.sinks - key0;
 #pragma unroll
@@ -1001,16 +1017,14 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
                     const bool page = !((none >> (i >> 3)) & 1u);
                     x[i] = page & (key < end) & ((key >= begin) | (key < sinks)) ? x[i] : -INFINITY;
                 }
-                top = top_of(x);
-                top = top == -INFINITY ? top : top * scale;
+                top = top_of(x) * scale;
             }
             if (__any(top > row_max + kGrow))
             {
                 const float m = fmaxf(row_max, top);
                 // (Before the first weight there is nothing but what is not finite.)
-                const float alpha = row_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
+                const float alpha = row_max == kNoMax ? 1.f : __builtin_amdgcn_exp2f(row_max - m);
                 row_max = m;
-                neg_max = m == -INFINITY ? 0.f : -m;
                 row_sum *= alpha;
 #pragma unroll
                 for (int d = 0; d < kDb; d++)
@@ -1024,25 +1038,27 @@ __global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const
         }
         key_now = key_next;
         key_next = key_third;
+        none = none_next;
     }
     // No load of this wave may be on its way into LDS when it ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (bad && c.status && lane == 0)
-        atomicOr(c.status, static_cast<int>(bad));
+    if (bad && c.status && tid == 0)
+        atomicOr(c.status, AWA_KV_BAD_PAGE);
     const float sum = sum_xor32(row_sum);
     if (wave_row0 + col >= rows)
         return;
-    const long long at = s.first + token;
+    const Row row = my_row();
+    const long long at = s.first + row.token;
     if (p.splits > 1)
     {
-        store_o(part_row(p, D, split, at, q_head), o, 1.f, half);
+        store_o(part_row(p, D, split, at, row.head), o, 1.f, half);
         if (half == 0)
-            *reinterpret_cast<float2*>(part_stats(p, D, split, at, q_head)) = make_float2(row_max, sum);
+            *reinterpret_cast<float2*>(part_stats(p, D, split, at, row.head)) = make_float2(sum == 0.f ? -INFINITY : row_max, sum);
         return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + at * p.out.stride +
-                               static_cast<long long>(q_head) * D * kElem;
+                               static_cast<long long>(row.head) * D * kElem;
     if (F32)
         store_o(reinterpret_cast<float*>(dst), o, inv, half);
     else

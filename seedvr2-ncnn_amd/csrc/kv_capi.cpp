@@ -53,6 +53,8 @@ int view(const awa_kv_cache* c, const awa_kv_rows* rows, int total, awa::KvView&
         return invalid("page_tokens must be a power of two from 16 to 1024");
     if (c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535)
         return invalid("the cache needs pages and 1 to 65535 heads");
+    if (static_cast<long long>(c->pages) * c->kv_heads * c->page_tokens > 0x7fffffffll)
+        return invalid("a pool has less than 2^31 rows");
     if (c->sequences <= 0 || c->sequences > 65535)
         return invalid("1 to 65535 sequences a call");
     if (c->table_width <= 0 || static_cast<long long>(c->table_width) * c->page_tokens > awa::kKvMaxSlots)

@@ -86,7 +86,7 @@ def rows(heads=2, total=3, size=2, dim=128, ptr=4096, **kw):
     return A.mat(ptr, dim, heads, total, size, dims=3, **kw)
 
 
-BAD_CACHES = [dict(fmt=2), dict(fmt=-1), dict(pages=0), dict(pages=-4), dict(page_tokens=8), dict(page_tokens=24),
+BAD_CACHES = [dict(fmt=2), dict(fmt=-1), dict(pages=0), dict(pages=-4), dict(pages=1 << 27, page_tokens=16, kv_heads=1), dict(page_tokens=8), dict(page_tokens=24),
               dict(page_tokens=2048), dict(page_tokens=0), dict(kv_heads=0), dict(kv_heads=70000), dict(head_dim=96),
               dict(head_dim=256), dict(sequences=0), dict(sequences=65536), dict(table_width=0),
               dict(table_width=1 << 27), dict(table_width=4, table_stride=3), dict(k=0), dict(v=0), dict(k=4104),
