@@ -616,7 +616,7 @@ __device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
 // are, in that order, what the lane holds of the PV product's operand P^T, and
 // V^T is read in the same key order.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(256, F32 || FOUR ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal, int part_tiles)
+__global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal, int part_tiles)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kRows = kTileRows;

@@ -9,9 +9,12 @@
 // Angles: positions of a long session are far from zero, so an angle's turns
 // are a 64-bit fraction times the position, of which the whole turns fall off
 // by overflow; the rest is within [-1/8, 1/8] turn of a quarter and goes
-// through the Taylor series of sine and cosine in 64 bits. The rotation is in
-// 64 bits too: a value next to a border of the 4-bit codes then falls where it
-// does in exact arithmetic.
+// through the Taylor series of sine and cosine in 64 bits. Rows that stay fp32
+// or become bf16 are rotated in fp32 with (cos, sin) rounded to fp32: off by at
+// most 2^-24 (|a| + 2 |b| + |r|) for r = a cos - b sin, far below half a step of
+// bf16. Keys that become four bits are rotated in 64 bits, and rounded once: a
+// value next to a border of the codes, of which a step is a third of the value,
+// then falls where it does in exact arithmetic.
 //
 // 4-bit rows: 32 features share a power of two 2^e, the least with max |x| <=
 // 7 * 2^e, so that no value is clipped by more than the half step that rounds
@@ -136,26 +139,43 @@ __device__ __forceinline__ Place place_row(const KvView& c, int t)
     return p;
 }
 
-// Index of a row in its pool.
+// Index of a row in its pool (of less than 2^31 rows).
 __device__ __forceinline__ size_t pool_row(const KvView& c, const Place& p, int head)
 {
-    return ((static_cast<size_t>(p.page) * c.heads + head) << c.page_shift) + (p.slot & ((1 << c.page_shift) - 1));
+    return static_cast<unsigned>(((p.page * c.heads + head) << c.page_shift) +
+                                 (p.slot & ((1 << c.page_shift) - 1)));
+}
+
+// Eight features as they lie in memory.
+template <bool F32>
+struct Raw8
+{
+    uint4 a, b;
+};
+
+template <bool F32>
+__device__ __forceinline__ Raw8<F32> load_raw(const unsigned char* p)
+{
+    Raw8<F32> r;
+    r.a = *reinterpret_cast<const uint4*>(p);
+    if (F32)
+        r.b = *reinterpret_cast<const uint4*>(p + 16);
+    return r;
 }
 
 template <bool F32>
-__device__ __forceinline__ void load8(const unsigned char* p, float (&v)[8])
+__device__ __forceinline__ void values8(const Raw8<F32>& r, float (&v)[8])
 {
     if (F32)
     {
-        const float4 a = *reinterpret_cast<const float4*>(p);
-        const float4 b = *reinterpret_cast<const float4*>(p + 16);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        v[0] = __uint_as_float(r.a.x), v[1] = __uint_as_float(r.a.y), v[2] = __uint_as_float(r.a.z);
+        v[3] = __uint_as_float(r.a.w), v[4] = __uint_as_float(r.b.x), v[5] = __uint_as_float(r.b.y);
+        v[6] = __uint_as_float(r.b.z), v[7] = __uint_as_float(r.b.w);
     }
     else
     {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
-        v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+        v[0] = bf16_lo(r.a.x), v[1] = bf16_hi(r.a.x), v[2] = bf16_lo(r.a.y), v[3] = bf16_hi(r.a.y);
+        v[4] = bf16_lo(r.a.z), v[5] = bf16_hi(r.a.z), v[6] = bf16_lo(r.a.w), v[7] = bf16_hi(r.a.w);
     }
 }
 
@@ -202,111 +222,165 @@ __device__ __forceinline__ void store8_four(unsigned char* codes, unsigned char*
         *scale = static_cast<unsigned char>(byte);
 }
 
+// How rows turn: not at all, neighbouring features, or the halves of a row.
+enum
+{
+    kStill,
+    kNeighbours,
+    kHalves
+};
+
+// a cos + b sin.
+__device__ __forceinline__ float turned(float a, float b, float c, float s)
+{
+    return fmaf(a, c, b * s);
+}
+
+__device__ __forceinline__ float turned(float a, float b, double c, double s)
+{
+    return round_odd(fma(static_cast<double>(a), c, static_cast<double>(b) * s));
+}
+
+// Eight features of a row, lane l of the row's; features behind the last pair
+// stay.
+template <int STYLE, int D, typename T2>
+__device__ __forceinline__ void rotate8(float (&v)[8], int l, int pairs, const T2* turn)
+{
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        x[e] = v[e];
+    if (STYLE == kNeighbours)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+        {
+            const T2 cs = turn[4 * l + e / 2];
+            v[e] = turned(x[e], x[e + 1], cs.x, -cs.y);
+            v[e + 1] = turned(x[e + 1], x[e], cs.x, cs.y);
+        }
+    }
+    else if (STYLE == kHalves)
+    {
+        // The other feature of each pair is `step` lanes away.
+        const int step = pairs / 8;
+        const bool second = l >= step;
+        const int from = l < 2 * step ? (second ? l - step : l + step) : 0;
+        const T2* const cs8 = turn + (l < 2 * step ? 8 * (second ? l - step : l) : 0);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+        {
+            const T2 cs = cs8[e];
+            v[e] = turned(x[e], __shfl(x[e], from, D / 8), cs.x, second ? cs.y : -cs.y);
+        }
+    }
+    if (STYLE && 2 * pairs < D)
+    {
+        const int left = 2 * pairs - 8 * l;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            v[e] = e < left ? v[e] : x[e];
+    }
+}
+
 // TOKENS tokens a workgroup and blockIdx.y's part of their heads; LANES lanes
-// hold a row, eight features each.
-template <bool F32, bool FOUR, int D, int TOKENS>
+// hold a row, eight features each. Bound by memory and, next, by the steps that
+// a row of 256 bytes takes (a quarter of a wave): queries, keys and values each
+// have a loop of their own, without a choice in it.
+template <bool F32, bool FOUR, int D, int TOKENS, int STYLE>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvAppendLaunch p, int heads_part)
 {
     constexpr int kLanes = D / 8;
     constexpr int kSlots = kThreads / kLanes; // rows at a time
     constexpr int kElem = F32 ? 4 : 2;
-    __shared__ double2 turn[TOKENS][kRopeMaxPairs];
+    __shared__ float2 turn[STYLE ? TOKENS : 1][kRopeMaxPairs];
+    __shared__ double2 exact_turn[STYLE && FOUR ? TOKENS : 1][kRopeMaxPairs];
     __shared__ Place places[TOKENS];
     const int tid = threadIdx.x;
-    const int wave = tid >> 6;
     const int t0 = blockIdx.x * TOKENS;
     const KvView& c = p.cache;
+    const int pairs = p.rope.pairs * p.rope.axes;
 
-    for (int i = wave; i < TOKENS; i += kThreads / 64)
+    for (int i = tid >> 6; i < TOKENS; i += kThreads / 64)
     {
+        const int lane = tid & 63;
         const Place at = t0 + i < c.total_rows ? place_row(c, t0 + i) : Place{-1, -1};
-        if ((tid & 63) == 0)
+        if (lane == 0)
             places[i] = at;
-        if (p.rope.axes > 0 && at.slot >= 0)
+        if (STYLE && at.slot >= 0 && lane < pairs)
         {
-            const int pair = tid & 63;
-            if (pair < p.rope.pairs * p.rope.axes)
-            {
-                const int axis = pair / p.rope.pairs;
-                const int x = p.positions ? p.positions[static_cast<long long>(t0 + i) * p.rope.axes + axis] : at.slot;
-                turn[i][pair] = cos_sin_turns(static_cast<unsigned long long>(static_cast<long long>(x)) *
-                                              p.rope.turns[pair - axis * p.rope.pairs]);
-            }
+            const int axis = lane / p.rope.pairs;
+            const int x = p.positions ? p.positions[static_cast<long long>(t0 + i) * p.rope.axes + axis] : at.slot;
+            const double2 cs = cos_sin_turns(static_cast<unsigned long long>(static_cast<long long>(x)) *
+                                             p.rope.turns[lane - axis * p.rope.pairs]);
+            turn[i][lane] = make_float2(static_cast<float>(cs.x), static_cast<float>(cs.y));
+            if (FOUR)
+                exact_turn[i][lane] = cs;
         }
     }
     __syncthreads();
     tell_status(c);
 
     const int l = tid % kLanes;
-    const int heads = (p.q.data ? p.q_heads : 0) + 2 * c.heads;
+    const int q_heads = p.q.data ? p.q_heads : 0;
     const int head0 = blockIdx.y * heads_part;
-    const int part = min(heads_part, heads - head0);
-    const int pairs = p.rope.pairs * p.rope.axes;
-    for (int i = tid / kLanes; i < TOKENS * part; i += kSlots)
-    {
-        const int token = i / part;
-        int head = head0 + i - token * part;
-        const Place at = places[token];
-        if (at.slot < 0)
-            continue;
-        // Queries first, then keys, then values.
-        const int q_heads = heads - 2 * c.heads;
-        const int kind = head < q_heads ? 0 : head < q_heads + c.heads ? 1 : 2;
-        head -= kind == 0 ? 0 : kind == 1 ? q_heads : q_heads + c.heads;
-        const KvRowsSource& src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-        const long long t = t0 + token;
-        float v[8];
-        load8<F32>(src.data + t * src.stride + (static_cast<long long>(head) * D + 8 * l) * kElem, v);
-        if (kind < 2 && p.rope.axes > 0)
+    // All rows of one kind, heads [first, first + count) of the launch's.
+    auto each_row = [&](int first, int count, const KvRowsSource& src, auto row) {
+        const int lo = max(head0 - first, 0);
+        const int n = min(head0 + heads_part - first, count) - lo;
+        if (n <= 0)
+            return;
+        int token = 0, head = lo + tid / kLanes;
+        while (true)
         {
-            float other[8];
-            int step = 0;
-            bool second = false;
-            if (p.rope.halves)
+            while (head >= lo + n && token < TOKENS)
             {
-                // The other feature of each pair is `step` lanes away.
-                step = pairs / 8;
-                second = l >= step;
-                const int from = l < 2 * step ? (second ? l - step : l + step) : l;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    other[e] = __shfl(v[e], from, kLanes);
+                head -= n;
+                token++;
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++)
+            if (token >= TOKENS)
+                return;
+            const Place at = places[token];
+            if (at.slot >= 0)
             {
-                const int f = 8 * l + e;
-                const int pair = p.rope.halves ? f - (second ? pairs : 0) : f >> 1;
-                const bool odd = p.rope.halves ? second : (e & 1) != 0;
-                if (f < 2 * pairs)
-                {
-                    const double2 cs = turn[token][pair];
-                    const double a = v[e];
-                    if (!p.rope.halves && !(e & 1))
-                        other[e + 1] = v[e], other[e] = v[e + 1];
-                    const double b = other[e];
-                    const double r = fma(a, cs.x, odd ? b * cs.y : -(b * cs.y));
-                    v[e] = F32 && kind == 0 ? static_cast<float>(r) : round_odd(r);
-                }
+                float v[8];
+                values8<F32>(load_raw<F32>(src.data + static_cast<long long>(t0 + token) * src.stride +
+                                           (head * D + 8 * l) * kElem),
+                             v);
+                row(v, at, token, head);
             }
+            head += kSlots;
         }
-        if (kind == 0)
-        {
-            store8<F32>(const_cast<unsigned char*>(p.q_out.data) + t * p.q_out.stride +
-                            (static_cast<long long>(head) * D + 8 * l) * kElem,
+    };
+    if (STYLE)
+        each_row(0, q_heads, p.q, [&](float (&v)[8], const Place&, int token, int head) {
+            rotate8<STYLE, D>(v, l, pairs, turn[token]);
+            store8<F32>(const_cast<unsigned char*>(p.q_out.data) +
+                            static_cast<long long>(t0 + token) * p.q_out.stride + (head * D + 8 * l) * kElem,
                         v);
-            continue;
-        }
-        if (at.page < 0)
-            continue;
-        const size_t row = pool_row(c, at, head);
-        unsigned char* const pool = kind == 1 ? c.k : c.v;
+        });
+    each_row(q_heads, c.heads, p.k, [&](float (&v)[8], const Place& at, int token, int head) {
         if (FOUR)
-            store8_four(pool + row * (D / 2) + 4 * l, (kind == 1 ? c.k_scale : c.v_scale) + row * (D / kKvGroup) + l / 4,
-                        l % 4 == 0, v);
+            rotate8<STYLE, D>(v, l, pairs, exact_turn[token]);
         else
-            store8<false>(pool + (row * D + 8 * l) * 2, v);
-    }
+            rotate8<STYLE, D>(v, l, pairs, turn[token]);
+        if (at.page < 0)
+            return;
+        const size_t r = pool_row(c, at, head);
+        if (FOUR)
+            store8_four(c.k + r * (D / 2) + 4 * l, c.k_scale + r * (D / kKvGroup) + l / 4, l % 4 == 0, v);
+        else
+            store8<false>(c.k + (r * D + 8 * l) * 2, v);
+    });
+    each_row(q_heads + c.heads, c.heads, p.v, [&](float (&v)[8], const Place& at, int, int head) {
+        if (at.page < 0)
+            return;
+        const size_t r = pool_row(c, at, head);
+        if (FOUR)
+            store8_four(c.v + r * (D / 2) + 4 * l, c.v_scale + r * (D / kKvGroup) + l / 4, l % 4 == 0, v);
+        else
+            store8<false>(c.v + (r * D + 8 * l) * 2, v);
+    });
 }
 
 // The other way: the rows that the cache holds at the new rows' slots. Rows
@@ -353,7 +427,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvReadLaunch p,
             four_values(word, unit, v);
         }
         else
-            load8<false>(pool + (row * D + 8 * l) * 2, v);
+            values8<false>(load_raw<false>(pool + (row * D + 8 * l) * 2), v);
         const KvRowsSource& to = key ? p.k : p.v;
         store8<F32>(const_cast<unsigned char*>(to.data) + (static_cast<long long>(t0) + token) * to.stride +
                         (static_cast<long long>(head) * D + 8 * l) * kElem,
@@ -379,13 +453,26 @@ Deal deal(int total, int heads, int head_dim)
     return d;
 }
 
+template <bool F32, bool FOUR, int D, int STYLE>
+void append_turned(const KvAppendLaunch& p, const Deal& d, hipStream_t stream)
+{
+    if (d.four_tokens)
+        hipLaunchKernelGGL((kv_append_kernel<F32, FOUR, D, 4, STYLE>), d.grid, dim3(kThreads), 0, stream, p,
+                           d.heads_part);
+    else
+        hipLaunchKernelGGL((kv_append_kernel<F32, FOUR, D, 1, STYLE>), d.grid, dim3(kThreads), 0, stream, p,
+                           d.heads_part);
+}
+
 template <bool F32, bool FOUR, int D>
 void append_to(const KvAppendLaunch& p, const Deal& d, hipStream_t stream)
 {
-    if (d.four_tokens)
-        hipLaunchKernelGGL((kv_append_kernel<F32, FOUR, D, 4>), d.grid, dim3(kThreads), 0, stream, p, d.heads_part);
+    if (p.rope.axes == 0)
+        append_turned<F32, FOUR, D, kStill>(p, d, stream);
+    else if (p.rope.halves)
+        append_turned<F32, FOUR, D, kHalves>(p, d, stream);
     else
-        hipLaunchKernelGGL((kv_append_kernel<F32, FOUR, D, 1>), d.grid, dim3(kThreads), 0, stream, p, d.heads_part);
+        append_turned<F32, FOUR, D, kNeighbours>(p, d, stream);
 }
 
 template <bool F32, bool FOUR, int D>

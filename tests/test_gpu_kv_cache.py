@@ -1,9 +1,12 @@
 """The key/value cache's kernels against their definitions in 64 bits.
 
-Tolerances: appended rows are rounded once from rotated values that are exact
-to about 2^-50, so pages must hold the very codes of the 64-bit result; rotated
-queries are off by half a step. Attention is bounded element by element
-(kv_model.attention)."""
+Tolerances: keys that become four bits are rounded once from rotated values that
+are exact to about 2^-50, so pages must hold the very codes of the 64-bit result,
+and so must values, which are not rotated. Rows that become bf16 or stay fp32 are
+rotated in fp32: r = a cos - b sin with cos, sin and one product rounded and the
+fused sum rounded is off by 2^-24 (|a cos| + 2 |b sin| + |r|), at most 2^-24 * 3
+(|a| + |b|), which comes to the half step of the type. Attention is bounded
+element by element (kv_model.attention)."""
 
 import ctypes
 
@@ -18,6 +21,17 @@ pytestmark = pytest.mark.gpu
 
 def new_rows(rng, counts, heads, dim, dtype, std=1.0):
     return M.as_type(rng.standard_normal((sum(counts), heads, dim)) * std, dtype)
+
+
+def rotation_bound(x, want, rope_dim, axes=1, halves=False, dtype="f32", **_):
+    """How far a row rotated in fp32 and stored as dtype may be from `want`."""
+    a = np.abs(np.asarray(x, np.float64))
+    both = np.zeros_like(a)
+    lo, hi = ((slice(0, rope_dim // 2), slice(rope_dim // 2, rope_dim)) if halves
+              else (slice(0, rope_dim, 2), slice(1, rope_dim, 2)))
+    both[..., lo] = both[..., hi] = a[..., lo] + a[..., hi]
+    fp32 = 3.0 * 2.0 ** -24 * both
+    return fp32 + (M.HALF[dtype] * (np.abs(want) + fp32) if dtype == "bf16" else 0.0)
 
 
 def expected_pools(cache, counts, k, v, skip=()):
@@ -54,8 +68,21 @@ def bf16_bits64(x):
     return A.f32_to_bf16_bits(odd.astype(np.uint32).view(np.float32))
 
 
-def check_pools(cache, want):
+def check_pools(cache, want, counts=None, k=None, rope=None):
+    """The pools; of bf16 pages the appended keys (k before the rotation) within
+    their bound, and all else to the bit."""
     got = cache.download()
+    if not cache.four and rope is not None:
+        at = 0
+        for s, n in enumerate(counts):
+            for j in range(n):
+                slot = int(cache.lengths[s]) - n + j
+                where = (cache.table[s, slot // cache.page], slice(None), slot % cache.page)
+                g, w = (A.bf16_bits_to_f32(x["k"][where]).astype(np.float64) for x in (got, want))
+                exact = rope["rows"][at + j]
+                assert (np.abs(g - exact) <= rotation_bound(k[at + j], exact, dtype="bf16", **rope["kw"])).all()
+                got["k"][where] = want["k"][where]
+            at += n
     for name, x in want.items():
         bad = np.argwhere(got[name] != x)
         assert len(bad) == 0, f"{name}: {len(bad)} of {x.size} differ, first at {bad[:3].tolist()}"
@@ -95,12 +122,13 @@ def test_append(gpu, dtype, fmt, rope, dim, heads, kv_heads, page):
         A.kv_append(desc, A.KvRows(40, cu.ptr), kd.blob, vd.blob, r, M_keep(pos), qd.blob, out.blob)
         kr = M.rotate(k, pos, **kw)
     A.synchronize()
-    check_pools(cache, expected_pools(cache, counts, kr, v.astype(np.float64)))
+    check_pools(cache, expected_pools(cache, counts, kr, v.astype(np.float64)), counts, k,
+                kw and {"rows": kr, "kw": kw})
     assert cache.status() == 0
     if kw is not None:
         got, want = out.read(), M.rotate(q, pos, **kw)
         n = sum(counts)
-        assert (np.abs(got[:n] - want[:n]) <= M.HALF[dtype] * np.abs(want[:n]) + 1e-12).all()
+        assert (np.abs(got[:n] - want[:n]) <= rotation_bound(q, want, dtype=dtype, **kw)[:n]).all()
         assert (got[n:] == 5.0).all()
         whole = out.read(whole=True)
         assert (whole[:, :16] == 7.0).all() and (whole[:, 16 + heads * dim:] == 7.0).all()
@@ -128,13 +156,14 @@ def test_append_far_positions(gpu, fmt):
     A.kv_append(desc, A.KvRows(len(pos)), kd.blob, vd.blob, A.Rope(128), M_keep(pos), qd.blob, qd.blob)  # in place
     want = M.rotate(q, pos, 128)
     # 2^31 positions of an angle that is exact to 2^-64 of a turn each.
-    assert (np.abs(qd.read() - want) <= M.HALF["f32"] * np.abs(want) + 2 * np.pi * 2.0 ** -33 * 2 * np.abs(q).max()).all()
+    assert (np.abs(qd.read() - want) <= rotation_bound(q, want, 128) + 2 * np.pi * 2.0 ** -33 * 2 * np.abs(q).max()).all()
 
     cache = M.Cache(fmt, [70], 2, 128, 16)
     desc = cache.upload()
     A.kv_append(desc, A.KvRows(len(pos)), kd.blob, vd.blob, A.Rope(126))
-    slots = np.arange(62, 70)[:, None]
-    check_pools(cache, expected_pools(cache, [8], M.rotate(k, slots, 126), v.astype(np.float64)))
+    kr = M.rotate(k, np.arange(62, 70)[:, None], 126)
+    check_pools(cache, expected_pools(cache, [8], kr, v.astype(np.float64)), [8], k,
+                {"rows": kr, "kw": {"rope_dim": 126}})
 
 
 def test_append_given_frequencies(gpu):
@@ -555,7 +584,6 @@ def test_a_session(gpu, fmt, dtype):
     cache.lengths[:] = 0
     desc = cache.upload()
     rope = A.Rope(126, 3)
-    held = {"k": [np.zeros((0, kv_heads, dim))] * 2, "v": [np.zeros((0, kv_heads, dim))] * 2}
     for counts, block in steps:
         total = sum(counts)
         q, k, v = (new_rows(rng, [total], h, dim, dtype) for h in (heads, kv_heads, kv_heads))
@@ -570,17 +598,11 @@ def test_a_session(gpu, fmt, dtype):
         A.kv_attention(desc, rows, qd.blob, mask, dim ** -0.5, out.blob, ws.ptr, n)
         A.synchronize()
         assert cache.status() == 0
-        kr, qr, got, at = M.rotate(k, pos, 126, 3), qd.read(), out.read(), 0
-        for s, c in enumerate(counts):
-            for name, x in (("k", kr), ("v", v.astype(np.float64))):
-                x = x[at:at + c]
-                new = M.decode4(*M.encode4(x)) if fmt == "4bit" else A.bf16_bits_to_f32(bf16_bits64(x)).astype(np.float64)
-                held[name][s] = np.concatenate([held[name][s], new.reshape(c, kv_heads, dim)])
-            if c:
-                want, bound = M.attention(qr[at:at + c], held["k"][s], held["v"][s], int(cache.lengths[s]), window,
-                                          sinks, block, dim ** -0.5, dtype)
-                assert (np.abs(got[at:at + c] - want) <= bound).all(), (counts, s)
-            at += c
+        kr = M.rotate(k, pos, 126, 3)
+        check_pools(cache, expected_pools(cache, counts, kr, v.astype(np.float64)), counts, k,
+                    {"rows": kr, "kw": {"rope_dim": 126, "axes": 3}})
+        cache.host = cache.download()
+        check_attention(cache, counts, qd.read(), dtype, out.read(), window, sinks, block)
 
 
 def hip():
