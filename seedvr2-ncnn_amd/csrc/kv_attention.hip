@@ -33,11 +33,10 @@ typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
 constexpr int kRowTile = 16;   // rows of kv_rows_kernel's tile
 constexpr int kTileRows = 128; // of kv_tile_kernel's
-constexpr int kTileShift = 5;  // and its keys
-constexpr int kTileKeys = 1 << kTileShift;
-constexpr int kKeyTile = 32;
-constexpr int kKeyShift = 5;
+constexpr int kKeyShift = 5;   // keys of both kernels' key tiles
+constexpr int kKeyTile = 1 << kKeyShift;
 constexpr int kWaves = 4;
+constexpr int kLongPart = 256; // key tiles of a part
 
 __device__ __forceinline__ float max_xor16(float x)
 {
@@ -110,17 +109,24 @@ __device__ __forceinline__ uint4 only_finite8(const uint4& v)
 }
 
 // A part's row and its (maximum, sum): all rows of part 0, of part 1, ..., then
-// the pairs.
-__device__ __forceinline__ float* part_row(const KvAttentionLaunch& p, int dim, int part, size_t row, int head)
+// the pairs. `row`: of part_index.
+__device__ __forceinline__ size_t part_index(const KvParts& k, int seq, const KvSequence& s, int token)
 {
-    const size_t all = static_cast<size_t>(p.cache.total_rows) * p.heads.d;
-    return p.partial + (part * all + row * p.heads.d + head) * dim;
+    return static_cast<size_t>(k.seq_rows > 0 ? static_cast<long long>(seq) * k.seq_rows : s.first) + token;
 }
 
-__device__ __forceinline__ float* part_stats(const KvAttentionLaunch& p, int dim, int part, size_t row, int head)
+__device__ __forceinline__ float* part_row(const KvAttentionLaunch& p, const KvParts& k, int dim, int part, size_t row,
+                                           int head)
 {
-    const size_t all = static_cast<size_t>(p.cache.total_rows) * p.heads.d;
-    return p.partial + p.splits * all * dim + (part * all + row * p.heads.d + head) * 2;
+    const size_t all = static_cast<size_t>(k.rows) * p.heads.d;
+    return k.partial + (part * all + row * p.heads.d + head) * dim;
+}
+
+__device__ __forceinline__ float* part_stats(const KvAttentionLaunch& p, const KvParts& k, int dim, int part, size_t row,
+                                             int head)
+{
+    const size_t all = static_cast<size_t>(k.rows) * p.heads.d;
+    return k.partial + k.splits * all * dim + (part * all + row * p.heads.d + head) * 2;
 }
 
 // One row tile of 16 rows, one part of its keys: each wave takes every fourth
@@ -137,7 +143,7 @@ __device__ __forceinline__ float* part_stats(const KvAttentionLaunch& p, int dim
 // matter as long as both operands agree: of 4-bit rows a lane has a quarter,
 // one load and one scale.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p, int two_tiles, int part_tiles)
+__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kChunks = D / 32;
@@ -150,14 +156,18 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     __shared__ float stats[kWaves][kRowTile][2];
 
     const KvView& c = p.cache;
-    const int seq = blockIdx.z;
+    const int seq = (blockIdx.y + blockIdx.z) % gridDim.y;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15;
     const int g = lane >> 4;
-    const int head = blockIdx.y;
-    const int tile = blockIdx.x & two_tiles; // one or two row tiles
-    const int split = blockIdx.x >> two_tiles;
+    // (Parts are in the slowest order, the last ones first, which only long
+    // sequences have: workgroups go to the XCDs in turn, and with parts in the
+    // fastest order one XCD got the first part of every sequence.)
+    const int tile = blockIdx.x / c.heads;
+    const int head = blockIdx.x - tile * c.heads;
+    const int split = p.one.splits - 1 - blockIdx.z;
+    const int part_tiles = p.one.part_tiles;
 
     const KvSequence s = kv_sequence(c, seq);
     if (s.bad && c.status && threadIdx.x == 0)
@@ -172,19 +182,20 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     const KvSpan span_last = kv_span(p.mask, slot0 + kv_divide(last, p.group), s.length);
     const KvTiles tiles = kv_tiles(span_first, span_last, kKeyShift);
     const int count = tiles.sinks + tiles.rest;
-    if (split * part_tiles >= count && p.splits > 1)
+    if (split * part_tiles >= count && p.one.splits > 1)
     {
         // No keys: the join leaves this part out.
         const int i = row0 + threadIdx.x;
         if (threadIdx.x < kRowTile && i <= last)
         {
             const int t = kv_divide(i, p.group);
-            part_stats(p, D, split, s.first + t, head * p.group.d + i - t * p.group.d)[0] = -INFINITY;
+            part_stats(p, p.one, D, split, part_index(p.one, seq, s, t), head * p.group.d + i - t * p.group.d)[0] =
+                -INFINITY;
         }
         return;
     }
     // (The last one takes all that is left: lengths may pass their bound.)
-    const int part_end = split + 1 == p.splits ? count : min(count, (split + 1) * part_tiles);
+    const int part_end = split + 1 == p.one.splits ? count : min(count, (split + 1) * part_tiles);
 
     // This lane's row (rows past the end repeat the last; they are not stored).
     const int row = min(row0 + r, last);
@@ -515,19 +526,19 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     }
     const int out_token = kv_divide(row0 + out_row, p.group);
     const int out_head = head * p.group.d + row0 + out_row - out_token * p.group.d;
-    const long long t = s.first + out_token;
-    if (p.splits > 1)
+    if (p.one.splits > 1)
     {
-        float* const dst = part_row(p, D, split, t, out_head) + f0;
+        const size_t at = part_index(p.one, seq, s, out_token);
+        float* const dst = part_row(p, p.one, D, split, at, out_head) + f0;
 #pragma unroll
         for (int e = 0; e < kPer; e++)
             dst[e] = v[e];
         if (f0 == 0)
-            *reinterpret_cast<float2*>(part_stats(p, D, split, t, out_head)) = make_float2(m, sum);
+            *reinterpret_cast<float2*>(part_stats(p, p.one, D, split, at, out_head)) = make_float2(m, sum);
         return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + t * p.out.stride +
+    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + static_cast<long long>(s.first + out_token) * p.out.stride +
                                (static_cast<long long>(out_head) * D + f0) * kElem;
 #pragma unroll
     for (int e = 0; e < kPer; e++)
@@ -586,8 +597,10 @@ __device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
     TileItem t;
     if (k < whole * d.each)
     {
-        t.unit = k % whole * 8 + xcd;
         t.part = q * d.each + k / whole;
+        // (An XCD's workgroups go to its four shader engines in turn: with a
+        // multiple of four units, a long sequence would be on one of them.)
+        t.unit = (k + (whole & 3 ? 0 : t.part)) % whole * 8 + xcd;
     }
     else
     {
@@ -616,12 +629,12 @@ __device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
 // are, in that order, what the lane holds of the PV product's operand P^T, and
 // V^T is read in the same key order.
 template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal, int part_tiles)
+__global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAttentionLaunch p, const TileDeal deal)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kRows = kTileRows;
     constexpr int kThreads = 256;
-    constexpr int kKeys = kTileKeys;
+    constexpr int kKeys = kKeyTile;
     constexpr int kC = D / 16;
     constexpr int kDb = D / 32;
     constexpr int kRowBytes = D * 2;
@@ -646,15 +659,18 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
         return;
     const int seq = item.unit / c.heads;
     const int head = item.unit - seq * c.heads;
-    const int split = item.part % p.splits;
-    const int tile = deal.parts / p.splits - 1 - item.part / p.splits;
 
     const KvSequence s = kv_sequence(c, seq);
     if (s.bad && c.status && tid == 0)
         atomicOr(c.status, static_cast<int>(s.bad));
     const int rows = s.rows * p.group.d;
+    const bool one = rows <= kRows;
+    const int splits = one ? p.one.splits : p.more.splits;
+    const int part_tiles = one ? p.one.part_tiles : p.more.part_tiles;
+    const int split = item.part % splits;
+    const int tile = (one ? 0 : p.tiles - 1) - item.part / splits;
     const int row0 = tile * kRows;
-    if (row0 >= rows)
+    if (tile < 0 || row0 >= rows)
         return;
     const int slot0 = s.length - s.rows;
     auto span_of = [&](int row) { return kv_span(p.mask, slot0 + kv_divide(row, p.group), s.length); };
@@ -709,17 +725,20 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
         }
     }
 
-    const KvTiles tiles = kv_tiles(first, last, kTileShift);
+    const KvTiles tiles = kv_tiles(first, last, kKeyShift);
     const int t_count = tiles.sinks + tiles.rest;
-    if (split * part_tiles >= t_count && p.splits > 1)
+    if (split * part_tiles >= t_count && splits > 1)
     {
         const Row row = my_row();
         if (half == 0 && wave_row0 + col < rows)
-            part_stats(p, D, split, s.first + row.token, row.head)[0] = -INFINITY;
+        {
+            const KvParts& k = one ? p.one : p.more;
+            part_stats(p, k, D, split, part_index(k, seq, s, row.token), row.head)[0] = -INFINITY;
+        }
         return;
     }
     const int t_begin = split * part_tiles;
-    const int t_end = split + 1 == p.splits ? t_count : min(t_count, t_begin + part_tiles);
+    const int t_end = split + 1 == splits ? t_count : min(t_count, t_begin + part_tiles);
 
     // A wave loads half a 16-key block of every tile.
     constexpr int kLoadRows = kKeys / 4;
@@ -728,7 +747,7 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     const int slot_mask = (1 << c.page_shift) - 1;
     auto tile_key = [&](int t) {
         t = min(t, t_end - 1);
-        return (t < tiles.sinks ? t : tiles.begin + t - tiles.sinks) << kTileShift;
+        return (t < tiles.sinks ? t : tiles.begin + t - tiles.sinks) << kKeyShift;
     };
     // The pages of a tile's two 16-key blocks, read a tile ahead. (A block behind
     // the last key has the last key's page; it is masked.)
@@ -1048,16 +1067,19 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     if (wave_row0 + col >= rows)
         return;
     const Row row = my_row();
-    const long long at = s.first + row.token;
-    if (p.splits > 1)
+    if (splits > 1)
     {
-        store_o(part_row(p, D, split, at, row.head), o, 1.f, half);
+        const KvParts& k = one ? p.one : p.more;
+        const size_t at = part_index(k, seq, s, row.token);
+        store_o(part_row(p, k, D, split, at, row.head), o, 1.f, half);
         if (half == 0)
-            *reinterpret_cast<float2*>(part_stats(p, D, split, at, row.head)) = make_float2(sum == 0.f ? -INFINITY : row_max, sum);
+            *reinterpret_cast<float2*>(part_stats(p, k, D, split, at, row.head)) =
+                make_float2(sum == 0.f ? -INFINITY : row_max, sum);
         return;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + at * p.out.stride +
+    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) +
+                               static_cast<long long>(s.first + row.token) * p.out.stride +
                                static_cast<long long>(row.head) * D * kElem;
     if (F32)
         store_o(reinterpret_cast<float*>(dst), o, inv, half);
@@ -1077,13 +1099,14 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
     const KvView& c = p.cache;
     const KvSequence s = kv_sequence(c, blockIdx.y);
     const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= s.rows * p.heads.d)
+    const KvParts k = !p.few && s.rows * p.group.d > kTileRows ? p.more : p.one;
+    if (k.splits == 1 || i >= s.rows * p.heads.d)
         return;
     const int lane = threadIdx.x & 63;
     const int token = kv_divide(i, p.heads);
     const int head = i - token * p.heads.d;
-    const size_t row = static_cast<size_t>(s.first) + token;
-    const float2 mine = lane < p.splits ? *reinterpret_cast<const float2*>(part_stats(p, D, lane, row, head))
+    const size_t row = part_index(k, blockIdx.y, s, token);
+    const float2 mine = lane < k.splits ? *reinterpret_cast<const float2*>(part_stats(p, k, D, lane, row, head))
                                         : make_float2(-INFINITY, 0.f);
     float m = mine.x;
 #pragma unroll
@@ -1109,7 +1132,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
             // (Past the last part: that one again, with no weight.)
             const int j = __builtin_amdgcn_readfirstlane(left ? __ffsll(left) - 1 : 0);
             const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j));
-            const float* const src = part_row(p, D, j, row, head) + lane * kPer;
+            const float* const src = part_row(p, k, D, j, row, head) + lane * kPer;
             by[b] = left ? w : 0.f;
 #pragma unroll
             for (int e = 0; e < kPer; e++)
@@ -1123,7 +1146,8 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
                 v[e] = fmaf(by[b], part[b][e], v[e]);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) + static_cast<long long>(row) * p.out.stride +
+    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) +
+                               static_cast<long long>(s.first + token) * p.out.stride +
                                static_cast<long long>(head) * D * (F32 ? 4 : 2);
 #pragma unroll
     for (int e = 0; e < kPer; e++)
@@ -1137,90 +1161,135 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
 
 } // namespace
 
-KvDeal kv_attention_deal(const KvView& c, int group, int head_dim, bool four, const KvMaskRule& mask, int max_length)
+void kv_attention_deal(KvAttentionLaunch& p, int max_length)
 {
-    const long long rows = static_cast<long long>(c.max_rows) * group;
-    KvDeal d;
-    d.few = rows <= 2 * kRowTile;
-    d.tile_rows = d.few ? kRowTile : kTileRows;
-    d.tiles = static_cast<int>((rows + d.tile_rows - 1) / d.tile_rows);
-    d.key_shift = d.few ? kKeyShift : kTileShift;
-    // Key tiles that a row tile may see, and the workgroups if none is split.
+    const KvView& c = p.cache;
+    const int group = p.group.d;
+    const int max_rows = std::min(c.max_rows, c.total_rows);
+    const long long rows = static_cast<long long>(max_rows) * group;
+    p.few = rows <= (p.four ? 3 : 1) * kRowTile;
+    const int tile_rows = p.few ? kRowTile : kTileRows;
+    p.tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+    // Key tiles that a row tile may see.
     long long keys = max_length;
-    if (mask.window > 0)
-        keys = std::min(keys, static_cast<long long>(mask.window) + mask.sinks + mask.block +
-                                  std::min(c.max_rows, d.tile_rows / group + 1));
-    const long long count = (keys >> d.key_shift) + 2;
-    const long long blocks = static_cast<long long>(d.tiles) * c.heads * c.sequences;
-    d.splits = 1;
-    if (d.few)
+    if (p.mask.window > 0)
+        keys = std::min(keys, static_cast<long long>(p.mask.window) + p.mask.sinks + p.mask.block +
+                                  std::min(max_rows, tile_rows / group + 1));
+    const long long count = (keys >> kKeyShift) + 2;
+    const auto parts = [&](long long splits) {
+        KvParts k{};
+        k.splits = static_cast<int>(std::max(1ll, std::min({splits, count, 64ll})));
+        k.part_tiles = static_cast<int>((count + k.splits - 1) / k.splits);
+        k.rows = c.total_rows;
+        return k;
+    };
+    // Few workgroups at the end would have the card to themselves: lengths may
+    // differ, so parts are not longer than this.
+    const long long least = (count + kLongPart - 1) / kLongPart;
+    if (p.few)
     {
         // The split with the least time, in key tiles of a workgroup: rounds of
         // workgroups (two or three a CU, by their registers), each with its start
         // and its part, and the join.
-        const long long slots = 256 * (four || head_dim == 64 ? 3 : 2);
-        long long best = 0;
-        for (int n = 1; n <= 64 && n <= count; n++)
+        const long long blocks = static_cast<long long>(p.tiles) * c.heads * c.sequences;
+        const long long slots = 256 * (p.four || p.head_dim == 64 ? 3 : 2);
+        long long best = -1, splits = 1;
+        for (long long n = std::min(least, 64ll); n <= 64 && n <= count; n++)
         {
             const long long part = (count + n - 1) / n;
             if (n > 1 && part < kWaves)
                 break;
             const long long time = (blocks * n + slots - 1) / slots * (part + 8) + (n > 1 ? 16 + n / 4 : 0);
-            if (n == 1 || time < best)
+            if (best < 0 || time < best)
             {
                 best = time;
-                d.splits = n;
+                splits = n;
             }
         }
+        p.one = p.more = parts(splits);
+        return;
     }
-    else if (blocks < 192)
-        // Too few to fill the device: two a CU, with at least eight key tiles.
-        d.splits = static_cast<int>(std::max(1ll, std::min({(511 + blocks) / blocks, count / 8, 64ll})));
-    d.part_tiles = static_cast<int>((count + d.splits - 1) / d.splits);
-    return d;
+    // Too few to fill the device: two a CU, with at least eight key tiles.
+    const auto fill = [&](long long blocks) {
+        return blocks < 192 ? std::min((511 + blocks) / blocks, count / 8) : 1;
+    };
+    if (p.tiles == 1)
+    {
+        p.one = p.more = parts(std::max(least, fill(static_cast<long long>(c.heads) * c.sequences)));
+        return;
+    }
+    // (A sequence's last row tile may have one row.)
+    const long long most = std::min(static_cast<long long>(p.tiles) * c.sequences,
+                                    static_cast<long long>(c.total_rows) * group / kTileRows + c.sequences);
+    p.more = parts(fill(c.heads * most));
+    // Single tokens and short chunks beside longer ones: if there can be any,
+    // they are dealt out by themselves.
+    p.one = parts(1);
+    const int one_rows = kTileRows / group;
+    if (one_rows > 0 && c.total_rows - (c.sequences - 1ll) * max_rows <= one_rows)
+    {
+        p.one = parts(std::max(least, fill(c.heads * (c.sequences - 1ll))));
+        p.one.seq_rows = one_rows;
+        p.one.rows = static_cast<long long>(one_rows) * c.sequences;
+    }
 }
 
-size_t kv_attention_partial_bytes(const KvView& c, int group, int head_dim, int splits)
+namespace
 {
-    return splits == 1 ? 0
-                       : static_cast<size_t>(c.total_rows) * c.heads * group * splits * (head_dim + 2) * sizeof(float);
+
+size_t partial_floats(const KvAttentionLaunch& p, const KvParts& k)
+{
+    return k.splits == 1 ? 0 : static_cast<size_t>(k.rows) * p.heads.d * k.splits * (p.head_dim + 2);
+}
+
+} // namespace
+
+size_t kv_attention_partial_bytes(const KvAttentionLaunch& p)
+{
+    return (partial_floats(p, p.one) + (p.tiles > 1 && !p.few ? partial_floats(p, p.more) : 0)) * sizeof(float);
+}
+
+void kv_attention_set_partial(KvAttentionLaunch& p, void* workspace)
+{
+    p.one.partial = static_cast<float*>(workspace);
+    p.more.partial = p.one.partial + (p.tiles > 1 && !p.few ? partial_floats(p, p.one) : 0);
 }
 
 namespace
 {
 
 template <int D, bool F32, bool FOUR>
-hipError_t launch(const KvAttentionLaunch& p, const KvDeal& d, hipStream_t stream)
+hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
 {
-    if (d.few)
+    if (p.few)
     {
-        const dim3 grid(d.tiles * d.splits, p.cache.heads, p.cache.sequences);
-        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p, d.tiles - 1,
-                           d.part_tiles);
+        const dim3 grid(p.tiles * p.cache.heads, p.cache.sequences, p.one.splits);
+        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p);
     }
     else
     {
-        const TileDeal t = tile_deal(p.cache.heads * p.cache.sequences, d.tiles * d.splits);
-        hipLaunchKernelGGL((kv_tile_kernel<D, F32, FOUR>), dim3(8u * t.period * t.periods), dim3(256), 0, stream, p, t,
-                           d.part_tiles);
+        const TileDeal t = tile_deal(p.cache.heads * p.cache.sequences,
+                                     std::max(p.tiles * p.more.splits, p.one.splits));
+        hipLaunchKernelGGL((kv_tile_kernel<D, F32, FOUR>), dim3(8u * t.period * t.periods), dim3(256), 0, stream, p, t);
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || d.splits == 1)
+    if (e != hipSuccess || (p.one.splits == 1 && p.more.splits == 1))
         return e;
-    hipLaunchKernelGGL((kv_merge_kernel<D, F32>),
-                       dim3((p.cache.max_rows * p.heads.d + 3) / 4, p.cache.sequences), dim3(256), 0, stream, p);
+    const int rows = p.more.splits > 1 ? p.cache.max_rows : std::min(p.cache.max_rows, p.one.seq_rows);
+    hipLaunchKernelGGL((kv_merge_kernel<D, F32>), dim3((rows * p.heads.d + 3) / 4, p.cache.sequences), dim3(256), 0,
+                       stream, p);
     return hipGetLastError();
 }
 
 } // namespace
 
-hipError_t launch_kv_attention(const KvAttentionLaunch& p, const KvDeal& d, hipStream_t stream)
+hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream)
 {
     if (p.head_dim == 128)
-        return p.four ? (p.f32 ? launch<128, true, true>(p, d, stream) : launch<128, false, true>(p, d, stream))
-                      : (p.f32 ? launch<128, true, false>(p, d, stream) : launch<128, false, false>(p, d, stream));
-    return p.four ? (p.f32 ? launch<64, true, true>(p, d, stream) : launch<64, false, true>(p, d, stream))
-                  : (p.f32 ? launch<64, true, false>(p, d, stream) : launch<64, false, false>(p, d, stream));
+        return p.four ? (p.f32 ? launch<128, true, true>(p, stream) : launch<128, false, true>(p, stream))
+                      : (p.f32 ? launch<128, true, false>(p, stream) : launch<128, false, false>(p, stream));
+    return p.four ? (p.f32 ? launch<64, true, true>(p, stream) : launch<64, false, true>(p, stream))
+                  : (p.f32 ? launch<64, true, false>(p, stream) : launch<64, false, false>(p, stream));
 }
 
 } // namespace awa

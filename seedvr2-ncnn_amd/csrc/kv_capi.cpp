@@ -125,7 +125,7 @@ int mask_rule(const awa_kv_mask* mask, awa::KvMaskRule& out)
 
 // Everything of an attention call but the buffers it writes.
 int attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob* q, const awa_kv_mask* mask,
-              awa::KvAttentionLaunch& p, awa::KvDeal& d)
+              awa::KvAttentionLaunch& p)
 {
     if (!cache)
         return invalid("null cache or rows");
@@ -148,9 +148,10 @@ int attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob
     const long long longest = mask->max_length > 0 && mask->max_length < slots ? mask->max_length : slots;
     if (static_cast<long long>(p.cache.max_rows) * q->h >= 1ll << 30)
         return invalid("max_rows times query heads must be below 2^30");
-    d = awa::kv_attention_deal(p.cache, group, p.head_dim, p.four, p.mask, static_cast<int>(longest));
-    p.splits = d.splits;
-    if (8ll * (static_cast<long long>(cache->sequences) * cache->kv_heads + 8) * (static_cast<long long>(d.tiles) * d.splits + 8) >= 1ll << 34)
+    awa::kv_attention_deal(p, static_cast<int>(longest));
+    if (8ll * (static_cast<long long>(cache->sequences) * cache->kv_heads + 8) *
+            (static_cast<long long>(p.tiles) * p.more.splits + p.one.splits + 8) >=
+        1ll << 34)
         return invalid("too many rows, heads and sequences for one call");
     return AWA_OK;
 }
@@ -283,10 +284,9 @@ int awa_kv_attention_workspace(const awa_kv_cache* cache, const awa_kv_rows* row
     if (!bytes)
         return invalid("null bytes");
     awa::KvAttentionLaunch p{};
-    awa::KvDeal d{};
-    const int rc = attention(cache, rows, q, mask, p, d);
+    const int rc = attention(cache, rows, q, mask, p);
     if (rc == AWA_OK)
-        *bytes = awa::kv_attention_partial_bytes(p.cache, p.group.d, p.head_dim, p.splits);
+        *bytes = awa::kv_attention_partial_bytes(p);
     return rc;
 }
 
@@ -294,8 +294,7 @@ int awa_kv_attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const a
                      float scale, const awa_blob* out, void* workspace, size_t workspace_bytes, void* stream)
 {
     awa::KvAttentionLaunch p{};
-    awa::KvDeal d{};
-    int rc = attention(cache, rows, q, mask, p, d);
+    int rc = attention(cache, rows, q, mask, p);
     if (rc == AWA_OK)
         rc = row_blob(out, "out", cache->head_dim, q->h, q->c, p.out);
     if (rc != AWA_OK)
@@ -305,11 +304,11 @@ int awa_kv_attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const a
     if (!std::isfinite(scale))
         return invalid("the scale must be finite");
     p.scale_log2 = scale * 1.44269504088896340736f;
-    const size_t need = awa::kv_attention_partial_bytes(p.cache, p.group.d, p.head_dim, p.splits);
+    const size_t need = awa::kv_attention_partial_bytes(p);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return invalid("this call needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
-    p.partial = static_cast<float*>(workspace);
-    return launched(awa::launch_kv_attention(p, d, static_cast<hipStream_t>(stream)), "kv attention kernel launch");
+    awa::kv_attention_set_partial(p, workspace);
+    return launched(awa::launch_kv_attention(p, static_cast<hipStream_t>(stream)), "kv attention kernel launch");
 }
 
 // What a row sees and how rows and keys are dealt out, on the host (tests).

@@ -172,6 +172,18 @@ struct KvReadLaunch
 };
 hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t stream);
 
+// How the key tiles of a row tile are dealt out: parts of part_tiles (the last
+// takes what lengths have beyond their bound).
+struct KvParts
+{
+    int splits, part_tiles;
+    // splits > 1: of every part the rows [D], unnormalised and relative to their
+    // maximum, by row and query head, then all (maximum, sum) pairs.
+    float* partial;
+    int seq_rows;   // rows that a sequence has room for, 0: as packed
+    long long rows; // of all sequences
+};
+
 struct KvAttentionLaunch
 {
     KvView cache;
@@ -182,26 +194,18 @@ struct KvAttentionLaunch
     KvRowsSource q, out;
     KvMaskRule mask;
     float scale_log2; // softmax scale * log2 e
-    int splits;       // parts that the keys of a row tile are dealt to
-    // splits > 1: per part, packed row and query head the unnormalised row
-    // [D] relative to its maximum, then all (maximum, sum) pairs.
-    float* partial;
+    bool few;         // rows: row tiles of 16, else of 128
+    int tiles;        // row tiles of the longest sequence
+    // Of sequences of one tile of 128 rows, and of longer ones.
+    KvParts one, more;
 };
 
-// How the work is dealt out: row tiles of one kernel or the other, and of each
-// the key tiles in parts of part_tiles, at most `splits`.
-struct KvDeal
-{
-    bool few; // rows: tiles of 16
-    int tile_rows, tiles; // rows of a row tile, row tiles of the longest sequence
-    int key_shift;
-    int splits, part_tiles;
-};
-
-// max_length: a bound of the lengths (the last part takes what longer ones have
-// beyond it).
-KvDeal kv_attention_deal(const KvView& cache, int group, int head_dim, bool four, const KvMaskRule& mask, int max_length);
-size_t kv_attention_partial_bytes(const KvView& cache, int group, int head_dim, int splits);
-hipError_t launch_kv_attention(const KvAttentionLaunch& p, const KvDeal& deal, hipStream_t stream);
+// Fills in how the work is dealt out (few and below). max_length: a bound of
+// the lengths.
+void kv_attention_deal(KvAttentionLaunch& p, int max_length);
+// Bytes of `one` and `more`'s parts, and where they are.
+size_t kv_attention_partial_bytes(const KvAttentionLaunch& p);
+void kv_attention_set_partial(KvAttentionLaunch& p, void* workspace);
+hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream);
 
 } // namespace awa

@@ -413,6 +413,49 @@ def test_attention(gpu, dtype, fmt, dim, case):
     check_attention(cache, counts, q, dtype, short, window, sinks, block)
 
 
+MIXED = [
+    # counts, lengths, heads, kv heads, window, sinks, bounds of the lengths
+    ([1, 200, 0, 3, 43, 42, 70], [5000, 300, 10, 2100, 90, 1500, 2000], 6, 2, 0, 0, (0, 5000, 5)),
+    ([128, 129, 1], [700, 700, 3000], 2, 2, 1100, 7, (0, 3000, 64)),
+    ([1, 2, 300], [9000, 2, 301], 4, 1, 0, 0, (0, 9000, 300)),
+    ([12, 1, 9], [800, 3000, 9], 4, 1, 0, 0, (0, 3000, 1)),
+    ([1, 2, 1], [400, 1300, 1], 140, 1, 0, 0, (0, 1300, 70)),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["bf16", "4bit"])
+@pytest.mark.parametrize("case", range(len(MIXED)))
+def test_single_tokens_beside_chunks(gpu, dtype, fmt, case):
+    """Sequences of few rows are dealt out otherwise than long ones of the same
+    call; a bound of the lengths that they pass changes only the split."""
+    counts, lengths, heads, kv_heads, window, sinks, bounds = MIXED[case]
+    rng = np.random.default_rng(40 + case)
+    cache = M.Cache(fmt, lengths, kv_heads, 64, 32, seed=case)
+    cache.upload()
+    q = new_rows(rng, [sum(counts) + 2], heads, 64, dtype, std=2.0)
+    for bound in bounds:
+        got = run_attention(cache, counts, q, dtype, window, sinks, max_length=bound)
+        check_attention(cache, counts, q, dtype, got, window, sinks)
+    assert cache.status() == 0
+
+
+def test_rows_bounds_above_the_rows(gpu):
+    """max_rows as a bound: sequences may all be shorter."""
+    rng = np.random.default_rng(46)
+    for counts, lengths, most in (([1, 2], [3000, 700], 500), ([3], [2000], 1000), ([150, 1], [160, 2500], 151)):
+        cache = M.Cache("bf16", lengths, 1, 64, 16)
+        cache.upload()
+        q = new_rows(rng, counts, 4, 64, "bf16")
+        qd, out = M.Rows(q, "bf16"), M.Rows(np.full(q.shape, 5.0), "bf16")
+        rows = A.KvRows(most, M_keep(np.cumsum([0] + counts)))
+        n = A.kv_attention_workspace(cache.desc, rows, qd.blob, A.KvMask())
+        ws = A.DeviceBuffer(max(n, 16))
+        A.kv_attention(cache.desc, rows, qd.blob, A.KvMask(), 0.125, out.blob, ws.ptr, n)
+        A.synchronize()
+        check_attention(cache, counts, q, "bf16", out.read())
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "4bit"])
 @pytest.mark.parametrize("counts,lengths", [([1, 3], [50, 40]), ([40, 70], [90, 70])])
 def test_what_masked_slots_hold_does_not_matter(gpu, fmt, counts, lengths):
