@@ -740,9 +740,11 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     const int t_begin = split * part_tiles;
     const int t_end = split + 1 == splits ? t_count : min(t_count, t_begin + part_tiles);
 
-    // A wave loads half a 16-key block of every tile.
-    constexpr int kLoadRows = kKeys / 4;
-    const int load_row = wave * kLoadRows;
+    // Of every tile a wave loads half a 16-key block; of 4-bit pages a block's
+    // keys or values.
+    constexpr int kLoadRows = FOUR ? 16 : kKeys / 4;
+    const int load_block = FOUR ? wave & 1 : wave >> 1;
+    const int load_row = FOUR ? 16 * load_block : wave * kLoadRows;
     constant_int* const table = (constant_int*)(c.table + static_cast<long long>(seq) * c.table_stride);
     const int slot_mask = (1 << c.page_shift) - 1;
     auto tile_key = [&](int t) {
@@ -767,7 +769,7 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     // The pool row of the wave's first row of the tile (pools have less than 2^31
     // rows).
     auto pool_row_of = [&](int key0, const Pages& pages, unsigned none) {
-        const int page = (none >> (wave >> 1)) & 1u ? 0 : wave < 2 ? pages.at[0] : pages.at[1];
+        const int page = (none >> load_block) & 1u ? 0 : load_block == 0 ? pages.at[0] : pages.at[1];
         return static_cast<size_t>(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(
             ((page * c.heads + head) << c.page_shift) + ((key0 + load_row) & slot_mask))));
     };
@@ -793,34 +795,56 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
             load_to_lds(v + j * 1024, l_row * kRowBytes + v_chunk(load_row + r, lane % kRowChunks) * 16, lds_v + at);
         }
     };
-    // 4-bit pages: a lane has 32 features of a key (the wave's first lanes) or of
-    // a value (the next ones), in registers until they go to LDS as bf16.
+    // 4-bit pages: two waves load a 16-key block of keys each, two of values, a
+    // lane 32 features of a row, in registers until they go to LDS as bf16. (Of
+    // 64 features half the lanes suffice. Lanes are dealt out so that eight in a
+    // row write to all banks.)
     constexpr int kGroups = D / 32;
-    constexpr int kFourLanes = kLoadRows * kGroups;
-    const int f_group = lane % kGroups;
-    const int f_row = lane / kGroups % kLoadRows;
-    const bool f_value = lane >= kFourLanes;
+    const bool f_value = wave >= 2;
+    const int f_row = D == 128 ? ((lane >> 1) & 3) + (lane >> 4) * 4
+                               : ((lane >> 1) & 3) * 2 + ((lane >> 3) & 1) + ((lane >> 4) & 1) * 8;
+    const int f_group = D == 128 ? (lane & 1) + ((lane >> 3) & 1) * 2 : lane & 1;
+    const uint32_t f_from = f_row * kGroups + f_group;
+    // Where a lane's four chunks go: chunk j at f_at ^ 16 j.
+    uint32_t f_at;
+    {
+        const int r = load_row + f_row;
+        const int low = D == 128 ? r & 3 : (r >> 1) & 3;
+        f_at = r * kRowBytes + ((f_value ? v_chunk(r, 4 * f_group) : k_chunk(r, 4 * f_group)) & ~3) * 16 + low * 16;
+    }
     uint4 codes;
     unsigned byte;
     auto load_four = [&](size_t pool_row) {
-        const size_t r = pool_row + f_row;
-        codes = *reinterpret_cast<const uint4*>((f_value ? c.v : c.k) + r * (D / 2) + 16 * f_group);
-        byte = (f_value ? c.v_scale : c.k_scale)[r * kGroups + f_group];
+        codes = *reinterpret_cast<const uint4*>((f_value ? c.v : c.k) + pool_row * (D / 2) + f_from * 16);
+        byte = ((f_value ? c.v_scale : c.k_scale) + pool_row * kGroups)[f_from];
     };
     auto store_four = [&](int slot) {
-        if (lane >= 2 * kFourLanes)
+        if (lane >= 16 * kGroups)
             return;
         const float unit = four_unit(byte);
-        const unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
-        const int r = load_row + f_row;
-        unsigned char* const dst = (f_value ? v_lds[slot] : k_lds[slot]) + r * kRowBytes;
+        unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
+        if (f_value)
+        {
+            // (The swizzle of V leaves the low bits of a chunk; written in order,
+            // four rows' chunks would share their banks.)
+#pragma unroll
+            for (int b = 1; b <= 2; b++)
+            {
+                const bool swap = f_at & (16 * b);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (!(j & b))
+                    {
+                        const unsigned x = words[j], y = words[j + b];
+                        words[j] = swap ? y : x;
+                        words[j + b] = swap ? x : y;
+                    }
+            }
+        }
+        unsigned char* const dst = f_value ? v_lds[slot] : k_lds[slot];
 #pragma unroll
         for (int j = 0; j < 4; j++)
-        {
-            const int chunk = 4 * f_group + j;
-            *reinterpret_cast<uint4*>(dst + (f_value ? v_chunk(r, chunk) : k_chunk(r, chunk)) * 16) =
-                four_bf16(words[j], unit);
-        }
+            *reinterpret_cast<uint4*>(dst + (f_at ^ (16 * j))) = four_bf16(words[j], unit);
     };
 
     f32x16 o[kDb];
