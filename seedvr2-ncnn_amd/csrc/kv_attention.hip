@@ -612,6 +612,84 @@ __device__ __forceinline__ TileItem tile_item(const TileDeal& d, int block)
     return t.part < d.parts ? t : TileItem{-1, 0};
 }
 
+// The sequence whose parts item `i` is among, by the whole wave: first[s] <= i <
+// first[s + 1].
+__device__ __forceinline__ int listed_sequence(const int* first, int sequences, int i)
+{
+    const int lane = threadIdx.x & 63;
+    int step = 1, s = 0;
+    while (step * 64 < sequences)
+        step *= 64;
+    for (;; step /= 64)
+    {
+        const int at = s + (lane + 1) * step;
+        s += __popcll(__ballot(at <= sequences && first[min(at, sequences)] <= i)) * step;
+        if (step == 1)
+            return __builtin_amdgcn_readfirstlane(s);
+    }
+}
+
+// Numbers the parts of all sequences (KvAttentionLaunch::list), by one workgroup.
+// (Sums stay below 2^30; behind what the grid has, they do not matter.)
+constexpr int kListThreads = 1024;
+__global__ __launch_bounds__(kListThreads) void kv_list_kernel(const KvAttentionLaunch p)
+{
+    constexpr long long kMost = 1ll << 30;
+    __shared__ long long sums[2][kListThreads / 64];
+    const KvView& c = p.cache;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    long long before[2] = {0, 0};
+    unsigned bad = 0;
+    for (int base = 0; base < c.sequences; base += kListThreads)
+    {
+        const int seq = base + threadIdx.x;
+        long long n[2] = {0, 0};
+        if (seq < c.sequences)
+        {
+            const KvSequence s = kv_sequence(c, seq);
+            const int rows = s.rows * p.group.d;
+            bad |= s.bad;
+            if (rows > kTileRows)
+                n[0] = static_cast<long long>((rows + kTileRows - 1) / kTileRows) * p.more.splits;
+            else if (rows > 0)
+                n[1] = p.one.splits;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+        {
+            const long long own = n[e];
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2)
+            {
+                const long long up = __shfl_up(n[e], off, 64);
+                n[e] += lane >= off ? up : 0;
+            }
+            if (lane == 63)
+                sums[e][wave] = n[e];
+            n[e] -= own;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+        {
+            long long all = 0;
+            for (int w = 0; w < kListThreads / 64; w++)
+            {
+                n[e] += w < wave ? sums[e][w] : 0;
+                all += sums[e][w];
+            }
+            if (seq < c.sequences)
+                p.list[e * (c.sequences + 1) + seq] = static_cast<int>(min(kMost, before[e] + n[e]));
+            before[e] = min(kMost, before[e] + all);
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x < 2)
+        p.list[threadIdx.x * (c.sequences + 1) + c.sequences] = static_cast<int>(before[threadIdx.x]);
+    if (bad && c.status)
+        atomicOr(c.status, static_cast<int>(bad));
+}
+
 // A tile of 128 rows, 32 a wave; key tiles of 32 go through LDS, which all
 // waves read. Bound by the matrix cores, and next by what feeds them: an operand
 // read from LDS serves one MFMA, so that MFMAs at full rate take all of LDS's
@@ -654,11 +732,25 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31;
     const int half = lane >> 5;
-    const TileItem item = tile_item(deal, blockIdx.x);
+    TileItem item = tile_item(deal, blockIdx.x);
     if (item.unit < 0)
         return;
-    const int seq = item.unit / c.heads;
-    const int head = item.unit - seq * c.heads;
+    int seq = 0, head = item.unit;
+    if (p.listed)
+    {
+        const int longer = __builtin_amdgcn_readfirstlane(p.list[c.sequences]);
+        const int* const first = p.list + (item.part < longer ? 0 : c.sequences + 1);
+        item.part -= item.part < longer ? 0 : longer;
+        if (item.part >= __builtin_amdgcn_readfirstlane(first[c.sequences]))
+            return;
+        seq = listed_sequence(first, c.sequences, item.part);
+        item.part -= __builtin_amdgcn_readfirstlane(first[seq]);
+    }
+    else
+    {
+        seq = item.unit / c.heads;
+        head = item.unit - seq * c.heads;
+    }
 
     const KvSequence s = kv_sequence(c, seq);
     if (s.bad && c.status && tid == 0)
@@ -668,7 +760,10 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     const int splits = one ? p.one.splits : p.more.splits;
     const int part_tiles = one ? p.one.part_tiles : p.more.part_tiles;
     const int split = item.part % splits;
-    const int tile = (one ? 0 : p.tiles - 1) - item.part / splits;
+    // (Tiles from the end, which see the most keys; unless listed, those of all
+    // sequences in step, so that the longest sequence's come first.)
+    const int tiles_all = one ? 1 : p.listed ? (rows + kRows - 1) / kRows : p.tiles;
+    const int tile = tiles_all - 1 - item.part / splits;
     const int row0 = tile * kRows;
     if (tile < 0 || row0 >= rows)
         return;
@@ -1122,64 +1217,66 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
     constexpr int kBatch = 8;
     const KvView& c = p.cache;
     const KvSequence s = kv_sequence(c, blockIdx.y);
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
     const KvParts k = !p.few && s.rows * p.group.d > kTileRows ? p.more : p.one;
-    if (k.splits == 1 || i >= s.rows * p.heads.d)
+    if (k.splits == 1)
         return;
     const int lane = threadIdx.x & 63;
-    const int token = kv_divide(i, p.heads);
-    const int head = i - token * p.heads.d;
-    const size_t row = part_index(k, blockIdx.y, s, token);
-    const float2 mine = lane < k.splits ? *reinterpret_cast<const float2*>(part_stats(p, k, D, lane, row, head))
-                                        : make_float2(-INFINITY, 0.f);
-    float m = mine.x;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1)
-        m = fmaxf(m, __shfl_xor(m, off, 64));
-    const bool there = mine.x != -INFINITY;
-    const float weight = there ? __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.f : m)) : 0.f;
-    float sum = there ? weight * mine.y : 0.f;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1)
-        sum += __shfl_xor(sum, off, 64);
-    unsigned long long left = __ballot(there);
-    float v[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; e++)
-        v[e] = 0.f;
-    while (left)
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < s.rows * p.heads.d; i += gridDim.x * 4)
     {
-        float part[kBatch][kPer], by[kBatch];
+        const int token = kv_divide(i, p.heads);
+        const int head = i - token * p.heads.d;
+        const size_t row = part_index(k, blockIdx.y, s, token);
+        const float2 mine = lane < k.splits ? *reinterpret_cast<const float2*>(part_stats(p, k, D, lane, row, head))
+                                            : make_float2(-INFINITY, 0.f);
+        float m = mine.x;
 #pragma unroll
-        for (int b = 0; b < kBatch; b++)
+        for (int off = 32; off >= 1; off >>= 1)
+            m = fmaxf(m, __shfl_xor(m, off, 64));
+        const bool there = mine.x != -INFINITY;
+        const float weight = there ? __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.f : m)) : 0.f;
+        float sum = there ? weight * mine.y : 0.f;
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1)
+            sum += __shfl_xor(sum, off, 64);
+        unsigned long long left = __ballot(there);
+        float v[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; e++)
+            v[e] = 0.f;
+        while (left)
         {
-            // (Past the last part: that one again, with no weight.)
-            const int j = __builtin_amdgcn_readfirstlane(left ? __ffsll(left) - 1 : 0);
-            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j));
-            const float* const src = part_row(p, k, D, j, row, head) + lane * kPer;
-            by[b] = left ? w : 0.f;
+            float part[kBatch][kPer], by[kBatch];
 #pragma unroll
-            for (int e = 0; e < kPer; e++)
-                part[b][e] = left ? src[e] : 0.f;
-            left &= left - 1;
+            for (int b = 0; b < kBatch; b++)
+            {
+                // (Past the last part: that one again, with no weight.)
+                const int j = __builtin_amdgcn_readfirstlane(left ? __ffsll(left) - 1 : 0);
+                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j));
+                const float* const src = part_row(p, k, D, j, row, head) + lane * kPer;
+                by[b] = left ? w : 0.f;
+#pragma unroll
+                for (int e = 0; e < kPer; e++)
+                    part[b][e] = left ? src[e] : 0.f;
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; b++)
+#pragma unroll
+                for (int e = 0; e < kPer; e++)
+                    v[e] = fmaf(by[b], part[b][e], v[e]);
         }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        unsigned char* const dst = const_cast<unsigned char*>(p.out.data) +
+                                   static_cast<long long>(s.first + token) * p.out.stride +
+                                   static_cast<long long>(head) * D * (F32 ? 4 : 2);
 #pragma unroll
-        for (int b = 0; b < kBatch; b++)
-#pragma unroll
-            for (int e = 0; e < kPer; e++)
-                v[e] = fmaf(by[b], part[b][e], v[e]);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    unsigned char* const dst = const_cast<unsigned char*>(p.out.data) +
-                               static_cast<long long>(s.first + token) * p.out.stride +
-                               static_cast<long long>(head) * D * (F32 ? 4 : 2);
-#pragma unroll
-    for (int e = 0; e < kPer; e++)
-    {
-        if (F32)
-            reinterpret_cast<float*>(dst)[lane * kPer + e] = v[e] * inv;
-        else
-            reinterpret_cast<__bf16*>(dst)[lane * kPer + e] = static_cast<__bf16>(v[e] * inv);
+        for (int e = 0; e < kPer; e++)
+        {
+            if (F32)
+                reinterpret_cast<float*>(dst)[lane * kPer + e] = v[e] * inv;
+            else
+                reinterpret_cast<__bf16*>(dst)[lane * kPer + e] = static_cast<__bf16>(v[e] * inv);
+        }
     }
 }
 
@@ -1189,8 +1286,7 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
 {
     const KvView& c = p.cache;
     const int group = p.group.d;
-    const int max_rows = std::min(c.max_rows, c.total_rows);
-    const long long rows = static_cast<long long>(max_rows) * group;
+    const long long rows = static_cast<long long>(c.max_rows) * group;
     p.few = rows <= (p.four ? 3 : 1) * kRowTile;
     const int tile_rows = p.few ? kRowTile : kTileRows;
     p.tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
@@ -1198,7 +1294,7 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
     long long keys = max_length;
     if (p.mask.window > 0)
         keys = std::min(keys, static_cast<long long>(p.mask.window) + p.mask.sinks + p.mask.block +
-                                  std::min(max_rows, tile_rows / group + 1));
+                                  std::min(c.max_rows, tile_rows / group + 1));
     const long long count = (keys >> kKeyShift) + 2;
     const auto parts = [&](long long splits) {
         KvParts k{};
@@ -1240,6 +1336,7 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
     if (p.tiles == 1)
     {
         p.one = p.more = parts(std::max(least, fill(static_cast<long long>(c.heads) * c.sequences)));
+        p.parts = p.one.splits;
         return;
     }
     // (A sequence's last row tile may have one row.)
@@ -1250,33 +1347,76 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
     // they are dealt out by themselves.
     p.one = parts(1);
     const int one_rows = kTileRows / group;
-    if (one_rows > 0 && c.total_rows - (c.sequences - 1ll) * max_rows <= one_rows)
+    if (one_rows > 0 && c.total_rows - (c.sequences - 1ll) * c.max_rows <= one_rows)
     {
         p.one = parts(std::max(least, fill(c.heads * (c.sequences - 1ll))));
-        p.one.seq_rows = one_rows;
-        p.one.rows = static_cast<long long>(one_rows) * c.sequences;
+        if (static_cast<long long>(one_rows) * c.sequences < c.total_rows)
+        {
+            p.one.seq_rows = one_rows;
+            p.one.rows = static_cast<long long>(one_rows) * c.sequences;
+        }
     }
+    // A workgroup without work takes about 0.8 ns of the launch, the list 4 us.
+    const long long each = std::max(static_cast<long long>(p.tiles) * p.more.splits, static_cast<long long>(p.one.splits));
+    const long long listed = static_cast<long long>(c.total_rows) * group / kTileRows * p.more.splits +
+                             static_cast<long long>(c.sequences) * std::max(p.one.splits, p.more.splits);
+    p.listed = (each * c.sequences - listed) * c.heads > 10000;
+    p.parts = p.listed ? listed : each;
 }
 
 namespace
 {
+
+TileDeal tile_deal(const KvAttentionLaunch& p)
+{
+    return tile_deal(p.cache.heads * (p.listed ? 1 : p.cache.sequences), static_cast<int>(p.parts));
+}
+
+// Workgroups of the join of a sequence's rows: one for four of them in a small
+// call, for many sequences no more than a single token needs.
+int merge_blocks(const KvAttentionLaunch& p)
+{
+    const long long rows = p.more.splits > 1 ? p.cache.max_rows : std::min(p.cache.max_rows, kTileRows / p.group.d);
+    return static_cast<int>(std::min((rows * p.heads.d + 3) / 4,
+                                     std::max((p.heads.d + 3ll) / 4, 8192ll / p.cache.sequences)));
+}
 
 size_t partial_floats(const KvAttentionLaunch& p, const KvParts& k)
 {
     return k.splits == 1 ? 0 : static_cast<size_t>(k.rows) * p.heads.d * k.splits * (p.head_dim + 2);
 }
 
-} // namespace
-
-size_t kv_attention_partial_bytes(const KvAttentionLaunch& p)
+size_t list_bytes(const KvAttentionLaunch& p)
 {
-    return (partial_floats(p, p.one) + (p.tiles > 1 && !p.few ? partial_floats(p, p.more) : 0)) * sizeof(float);
+    return p.listed ? (2 * (p.cache.sequences + 1) * sizeof(int) + 15) / 16 * 16 : 0;
 }
 
-void kv_attention_set_partial(KvAttentionLaunch& p, void* workspace)
+} // namespace
+
+size_t kv_attention_workspace_bytes(const KvAttentionLaunch& p)
 {
-    p.one.partial = static_cast<float*>(workspace);
+    return list_bytes(p) +
+           (partial_floats(p, p.one) + (p.tiles > 1 && !p.few ? partial_floats(p, p.more) : 0)) * sizeof(float);
+}
+
+void kv_attention_set_workspace(KvAttentionLaunch& p, void* workspace)
+{
+    p.list = static_cast<int*>(workspace);
+    p.one.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + list_bytes(p));
     p.more.partial = p.one.partial + (p.tiles > 1 && !p.few ? partial_floats(p, p.one) : 0);
+}
+
+bool kv_attention_fits(const KvAttentionLaunch& p)
+{
+    const long long most = 1ll << 23; // workgroups of a launch: their threads are counted in 32 bits
+    if (p.heads.d / 4 >= most || static_cast<long long>(p.cache.heads) * p.cache.sequences >= most)
+        return false;
+    if (p.few)
+        return static_cast<long long>(p.tiles) * p.cache.heads < most;
+    if (p.parts >= most)
+        return false;
+    const TileDeal t = tile_deal(p);
+    return 8ll * t.period * t.periods < most;
 }
 
 namespace
@@ -1292,16 +1432,21 @@ hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
     }
     else
     {
-        const TileDeal t = tile_deal(p.cache.heads * p.cache.sequences,
-                                     std::max(p.tiles * p.more.splits, p.one.splits));
+        if (p.listed)
+        {
+            hipLaunchKernelGGL(kv_list_kernel, dim3(1), dim3(kListThreads), 0, stream, p);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess)
+                return e;
+        }
+        const TileDeal t = tile_deal(p);
         hipLaunchKernelGGL((kv_tile_kernel<D, F32, FOUR>), dim3(8u * t.period * t.periods), dim3(256), 0, stream, p, t);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || (p.one.splits == 1 && p.more.splits == 1))
         return e;
-    const int rows = p.more.splits > 1 ? p.cache.max_rows : std::min(p.cache.max_rows, p.one.seq_rows);
-    hipLaunchKernelGGL((kv_merge_kernel<D, F32>), dim3((rows * p.heads.d + 3) / 4, p.cache.sequences), dim3(256), 0,
-                       stream, p);
+    hipLaunchKernelGGL((kv_merge_kernel<D, F32>), dim3(merge_blocks(p), p.cache.sequences),
+                       dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

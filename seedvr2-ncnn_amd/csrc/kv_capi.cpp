@@ -70,6 +70,8 @@ int view(const awa_kv_cache* c, const awa_kv_rows* rows, int total, awa::KvView&
         return invalid("4-bit pages need 4-byte aligned scale pools");
     if (rows->max_rows <= 0 || rows->max_rows > awa::kKvMaxSlots)
         return invalid("max_rows must be 1 to 2^30");
+    if (total > 1 << 25)
+        return invalid("a call takes at most 2^25 rows");
     if (!rows->cu_rows && static_cast<long long>(rows->max_rows) * c->sequences != total)
         return invalid("without cu_rows the blobs must hold max_rows rows for every sequence");
     int shift = 0;
@@ -149,9 +151,7 @@ int attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_blob
     if (static_cast<long long>(p.cache.max_rows) * q->h >= 1ll << 30)
         return invalid("max_rows times query heads must be below 2^30");
     awa::kv_attention_deal(p, static_cast<int>(longest));
-    if (8ll * (static_cast<long long>(cache->sequences) * cache->kv_heads + 8) *
-            (static_cast<long long>(p.tiles) * p.more.splits + p.one.splits + 8) >=
-        1ll << 34)
+    if (!awa::kv_attention_fits(p))
         return invalid("too many rows, heads and sequences for one call");
     return AWA_OK;
 }
@@ -286,7 +286,7 @@ int awa_kv_attention_workspace(const awa_kv_cache* cache, const awa_kv_rows* row
     awa::KvAttentionLaunch p{};
     const int rc = attention(cache, rows, q, mask, p);
     if (rc == AWA_OK)
-        *bytes = awa::kv_attention_partial_bytes(p);
+        *bytes = awa::kv_attention_workspace_bytes(p);
     return rc;
 }
 
@@ -304,10 +304,10 @@ int awa_kv_attention(const awa_kv_cache* cache, const awa_kv_rows* rows, const a
     if (!std::isfinite(scale))
         return invalid("the scale must be finite");
     p.scale_log2 = scale * 1.44269504088896340736f;
-    const size_t need = awa::kv_attention_partial_bytes(p);
+    const size_t need = awa::kv_attention_workspace_bytes(p);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return invalid("this call needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
-    awa::kv_attention_set_partial(p, workspace);
+    awa::kv_attention_set_workspace(p, workspace);
     return launched(awa::launch_kv_attention(p, static_cast<hipStream_t>(stream)), "kv attention kernel launch");
 }
 

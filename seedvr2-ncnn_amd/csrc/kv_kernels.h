@@ -198,14 +198,22 @@ struct KvAttentionLaunch
     int tiles;        // row tiles of the longest sequence
     // Of sequences of one tile of 128 rows, and of longer ones.
     KvParts one, more;
+    // Where many sequences are far shorter than the longest, the parts of all of
+    // them are numbered through, `parts` at most: first those of longer
+    // sequences, then those of one tile. Of both the number of the first part by
+    // sequence, [2][sequences + 1].
+    bool listed;
+    long long parts; // else: of every sequence
+    int* list;
 };
 
 // Fills in how the work is dealt out (few and below). max_length: a bound of
 // the lengths.
 void kv_attention_deal(KvAttentionLaunch& p, int max_length);
-// Bytes of `one` and `more`'s parts, and where they are.
-size_t kv_attention_partial_bytes(const KvAttentionLaunch& p);
-void kv_attention_set_partial(KvAttentionLaunch& p, void* workspace);
+bool kv_attention_fits(const KvAttentionLaunch& p); // its grids can be launched
+// Bytes of the list and of `one` and `more`'s parts, and where they are.
+size_t kv_attention_workspace_bytes(const KvAttentionLaunch& p);
+void kv_attention_set_workspace(KvAttentionLaunch& p, void* workspace);
 hipError_t launch_kv_attention(const KvAttentionLaunch& p, hipStream_t stream);
 
 } // namespace awa

@@ -140,7 +140,10 @@ class Cache:
         slot = np.arange(length)
         page = self.table[s, slot // self.page] if length else np.zeros(0, int)
         ok = (page >= 0) & (page < self.pages)
-        return self.values(name)[np.where(ok, page, 0), :, slot % self.page], ok
+        at = np.where(ok, page, 0), slice(None), slot % self.page
+        if self.four:
+            return decode4(self.host[name][at], self.host[name + "_scale"][at]), ok
+        return A.bf16_bits_to_f32(self.host[name][at]).astype(np.float64), ok
 
     def upload(self, spare=0):
         for name, x in {**self.host, "table": self.table, "lengths": self.lengths,

@@ -440,6 +440,30 @@ def test_single_tokens_beside_chunks(gpu, dtype, fmt, case):
     assert cache.status() == 0
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "4bit"])
+def test_many_single_tokens_beside_a_chunk(gpu, fmt):
+    """Parts numbered through over sequences of 0, 1, a few and many rows, some of
+    which do not fit together: more than a wave's and more than a workgroup's."""
+    rng = np.random.default_rng(47)
+    for n, most, heads, kv_heads in ((100, 700, 8, 4), (1500, 300, 2, 1), (70, 900, 6, 2)):
+        counts = [1] * n
+        for s, x in ((0, 0), (1, 40), (n // 2, most), (n - 3, 129), (n - 2, 0), (n - 1, 3)):
+            counts[s] = x
+        lengths = [int(x) + c for x, c in zip(rng.integers(0, 60, n), counts)]
+        lengths[2], lengths[n // 2 + 1] = 3000, 1500
+        cache = M.Cache(fmt, lengths, kv_heads, 64, 16)
+        cache.lengths[5] = 0                      # below its new rows
+        cache.lengths[6] = cache.table.shape[1] * 16 + 1
+        cache.upload()
+        q = new_rows(rng, [sum(counts) + 1], heads, 64, "bf16", std=2.0)
+        for bound in (0, 3000):
+            got = run_attention(cache, counts, q, "bf16", max_length=bound)
+            check_attention(cache, counts, q, "bf16", got, sequences=set(range(n)) - {5, 6})
+            for s in (5, 6):
+                assert (got[sum(counts[:s])] == 5.0).all()
+        assert cache.status() == A.KV_BAD_LENGTH
+
+
 def test_rows_bounds_above_the_rows(gpu):
     """max_rows as a bound: sequences may all be shorter."""
     rng = np.random.default_rng(46)

@@ -186,6 +186,42 @@ def test_workspace_is_asked_for():
     assert A.kv_attention_workspace(c, r, q, A.KvMask(max_length=64)) == 0
 
 
+def test_workspace_of_single_tokens_beside_chunks():
+    """Parts are kept of a call's rows alone, however many sequences it has, and
+    of sequences of one row tile alone where longer ones fill the device."""
+    def bytes_of(sequences, total, most, max_length, heads=8, kv_heads=2):
+        c = cache(kv_heads=kv_heads, sequences=sequences, table_width=8192)
+        return A.kv_attention_workspace(c, A.KvRows(most, 4096), rows(heads=heads, total=total), A.KvMask(max_length=max_length))
+
+    part = 8 * 130 * 4  # a row of a part, of all heads, bytes
+    # Chunks of many row tiles, which are not split: none can have few rows.
+    assert bytes_of(60, 60 * 500, 500, 60000) == 0
+    for sequences, total, most in ((2, 4097, 4096), (60, 5000, 4096), (60, 700, 300), (1000, 5095, 4096)):
+        n = bytes_of(sequences, total, most, 60000)
+        numbers = -(-2 * (sequences + 1) * 4 // 16) * 16  # of the parts' list
+        assert n > 0 and (n % part == 0 or (n - numbers) % part == 0)
+        assert n <= 2 * 64 * part * total + numbers
+    # Of 1000 sequences at most 32 rows of each are in one row tile.
+    assert bytes_of(1000, 10 ** 6, 9 * 10 ** 5, 60000) <= 64 * part * 32000 + 10 ** 4
+
+
+def test_calls_of_too_many_workgroups_are_refused():
+    def ask(sequences, total, most, kv_heads, heads, max_length=0):
+        c = cache(kv_heads=kv_heads, sequences=sequences, table_width=1024)
+        return A.kv_attention_workspace(c, A.KvRows(most, 4096), rows(heads=heads, total=total), A.KvMask(max_length=max_length))
+
+    assert ask(65535, 65535, 1, 20, 20, 64) == 0
+    # Many short sequences beside a long one: numbered through, not all as long.
+    for sequences, most, heads in ((4000, 16384, 32), (65535, 4096, 24)):
+        assert ask(sequences, most + sequences - 1, most, 8, heads, 64) < 10 ** 6
+    for args in ((65535, 65535, 1, 65535, 65535), (65535, 1 << 25, 500, 300, 300), (1, 1 << 24, 1 << 24, 8, 64),
+                 (1, 1 << 22, 1 << 22, 300, 300), (2, 2, 1, 1, 1 << 30)):
+        refused(lambda: ask(*args))
+    big = rows(total=(1 << 25) + 1)
+    refused(lambda: A.kv_append(cache(), A.KvRows(5, 4096), big, big))
+    refused(lambda: A.kv_read(cache(), A.KvRows(5, 4096), big, big))
+
+
 @pytest.mark.parametrize("args", [(0,), (130,), (7,), (128, 5), (-2,), (64, 0), (12, 3, -1.0), (128, 1, 0.0),
                                   (128, 1, float("nan")), (128, 1, float("inf")), (126, 3, 1e4, True), (24, 1, 1e4, True)])
 def test_rope_refusals(args):
