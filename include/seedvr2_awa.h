@@ -445,7 +445,8 @@ int awa_dit_stack_block_times(const awa_dit_stack* stack, float* block_ms);
  *   AWA_KV_BAD_LENGTH: a length is negative, beyond the page table row, or
  *     below the sequence's new rows; AWA_KV_BAD_ROWS: its rows in cu_rows are
  *     out of order, beyond the blobs, or more than max_rows. Such a sequence
- *     takes no part in the call.
+ *     takes no part in the call, and what becomes of rows that two sequences
+ *     then claim is open.
  * Table entries behind a sequence's length are not read. Sequences may share
  * pages, but not append to one slot in one call (either row may win). Rows of
  * blobs behind the last sequence's are left as they were. Nothing is
@@ -473,8 +474,9 @@ typedef struct awa_kv_cache {
 } awa_kv_cache;
 
 /* The new rows in the packed blobs: sequence s has rows [cu_rows[s],
- * cu_rows[s + 1]) (device, sequences + 1 ints), at most max_rows. cu_rows null:
- * max_rows each. */
+ * cu_rows[s + 1]) (device, sequences + 1 ints), at most max_rows; single tokens
+ * of some sequences may stand beside long chunks of others. cu_rows null:
+ * max_rows each. A call takes 1 to 2^25 rows. */
 typedef struct awa_kv_rows {
     const int* cu_rows;
     int max_rows;
@@ -502,6 +504,9 @@ void awa_rope_destroy(awa_rope* rope);
 
 /* Appends new rows: k, rotated, and v into the pages (rounded once, to the
  * cache's format); q, rotated, to q_out (q itself, or memory apart from it).
+ * Keys that become four bits are rotated in 64 bits; what becomes bf16 or stays
+ * fp32 is rotated in fp32, a cos - b sin off by at most 2^-24 * 3 (|a| + |b|)
+ * before it is rounded to its type.
  * Mats (head_dim, heads, rows) of one type, fp32 or bf16, rows (cstep) at
  * 16-byte addresses, so views of a fused QKV projection will do. rope null:
  * keys go in as they are and there is no q. positions: device ints
@@ -522,8 +527,8 @@ int awa_kv_read(const awa_kv_cache* cache, const awa_kv_rows* rows, const awa_bl
  * block 1 is causal attention (e = p + 1). block > 1: blocks of that many
  * slots behind the sinks see each other, as the tokens of a frame do.
  * max_length: an upper bound of the lengths, 0 for all that a page table row
- * can name. It sets how far the work is split; longer sequences are still
- * right. */
+ * can name. It sets how far the work is split and the workspace: best near the
+ * longest; longer sequences are still right. */
 typedef struct awa_kv_mask {
     int window; /* 0: unlimited */
     int sinks;
@@ -535,8 +540,9 @@ typedef struct awa_kv_mask {
  * Mats (head_dim, heads, rows) of one type, heads a multiple of kv_heads (query
  * head h reads key/value head h / (heads / kv_heads)). fp32 statistics and
  * sums; bf16 rows round probabilities to bf16, fp32 rows keep 24 bits of
- * queries and probabilities. A row that sees nothing gives zeros; what masked
- * slots hold (NaN too) does not matter. out may be q.
+ * queries and probabilities. A row that sees nothing, or whose scores are all
+ * -inf, gives zeros; what masked slots hold (NaN too) does not matter. The same
+ * call gives the same bits every time. out may be q.
  * workspace: device memory of awa_kv_attention_workspace bytes for the same
  * arguments, 16-byte aligned, for this call alone while it runs (calls on
  * other streams, and captured graphs that may run beside each other, need

@@ -5,14 +5,15 @@
 // a row sees, in one pass with the running maximum m. The rows of one sequence
 // that share a key/value head (its new tokens times the query heads of a
 // group) are packed into row tiles; the key tiles that a row tile sees (those
-// of the sinks, then those of the window) are dealt to `splits` workgroups,
-// whose parts kv_merge_kernel joins.
+// of the sinks, then those of the window) are dealt to one or several
+// workgroups, whose parts kv_merge_kernel joins.
 //
 // fp32 rows: queries and probabilities are three bf16 pieces (all 24 bits), so
 // that products with the cache's values are exact and sums are fp32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -134,7 +135,12 @@ __device__ __forceinline__ float* part_stats(const KvAttentionLaunch& p, const K
 // operand registers and V through the wave's own LDS, from which it is read
 // transposed; the waves' results are joined at the end. Bound by reading the
 // cache: the next tile's rows are asked for as soon as this one's registers are
-// free.
+// free. One row over 131072 keys of 20 heads of 128, bf16: 227 us with the join,
+// 5.9 TB/s; 32 rows of up to 16384 keys over four bits 166 us, 5.0 TB/s, where
+// unpacking the codes shares the vector units with the softmax. (Eight or sixteen
+// waves a workgroup and registers for three or four workgroups a CU were slower,
+// as were chunks of V in an order that frees LDS of bank conflicts: 36.5 us to
+// 35.9 for bf16 rows of 16 sequences of 8000 keys, 31.2 to 32.3 for fp32 ones.)
 //
 // S^T = K Q^T (16x16x32): lane (r = lane % 16, g = lane / 16) holds row r's
 // scores of keys 4 g + [0, 4) of each 16. Those of two blocks are, in that
@@ -696,11 +702,15 @@ __global__ __launch_bounds__(kListThreads) void kv_list_kernel(const KvAttention
 // bandwidth. Three workgroups share a CU (two of fp32 rows, whose queries take
 // three times the registers), so that one's softmax, waits and edges run beside
 // the others' products: nothing else of the loop overlaps by itself, and
-// schedules within a wave gained less. 16384 rows of 20 heads, 128 features: 1420
-// us so (950 TFLOP/s), 1426 with two workgroups that take the scores of the next
-// block beside a block's softmax, 1557 with one such of eight waves, whose
-// barriers keep them in step, 1834 with four waves of 64 rows, which read half
-// the operands but leave a matrix core one wave to be fed by.
+// schedules within a wave gained less. 16384 rows of 20 heads, 128 features,
+// causal: 1300 us so (1.04 PFLOP/s; a matrix product of 8192^3 reaches 1.2), the
+// matrix cores and the vector units busy for half of it each. Two workgroups that
+// take the scores of the next block beside a block's softmax: 1440 us; one such
+// of eight waves, whose barriers keep them in step: 1557; four waves of 64 rows,
+// which read half the operands but leave a matrix core one wave to be fed by:
+// 1834. Without its loads of keys and values the loop would take 1183 us, without
+// the exponentials 1244, without half of its LDS reads 1270: no single part
+// bounds it.
 //
 // S^T = K Q^T (32x32x16): lane (col = lane % 32, half = lane / 32) holds row
 // col's scores of keys 8 (i / 4) + 4 half + i % 4, i < 16; eight of them in a row
@@ -1208,8 +1218,9 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
 
 // Joins the parts of a row: M = max m_i, out = sum 2^(m_i - M) o_i / sum
 // 2^(m_i - M) l_i, in the parts' order; parts without a key are left out. One
-// wave a row and query head. Bound by latency: all parts' maxima and sums come
-// with one load, their rows with independent ones.
+// wave a row and query head at a time. Bound by latency: all parts' maxima and
+// sums come with one load, their rows with independent ones, eight at a time.
+// 3.2 us for 20 rows, 3.6 us for 2048.
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p)
 {
@@ -1282,11 +1293,56 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
 
 } // namespace
 
+namespace
+{
+
+// Parts of a row tile of 128 rows with the least time for `blocks` of them, which
+// see `count` key tiles on the average. Measured, in us a key tile: a workgroup that
+// has a CU to itself, and a CU's full set of them side by side (which a CU takes
+// set after set; of the last one it has a part); a part's rows are written and
+// read again. 8 heads of 128 over 8000 keys (us): 8 workgroups 198, split 28;
+// 64 (1024 rows) 191, split 58. 20 heads: 220 (1408 rows over 31408 keys) 728, in
+// three parts 504; 320 (2048 over 8048) 218, in two 204; 460 265, in two 322; 100
+// (640 over 640) 26, in two 31.
+long long tile_splits(const KvAttentionLaunch& p, long long blocks, long long block_rows, double count)
+{
+    const bool half = p.head_dim == 64;
+    const double alone = (p.f32 ? 1.35 : p.four ? 1.0 : 0.75) * (half ? 0.85 : 1.0);
+    const double full = (p.f32 ? 1.8 : p.four ? 1.7 : 1.55) * (half ? 0.9 : 1.0);
+    const int set = p.f32 ? (half && !p.four ? 3 : 2) : half ? 4 : 3;
+    const double join = 0.045 * block_rows / kTileRows * p.head_dim / 128;
+    const auto time = [&](long long n) {
+        const double each = blocks * n / 256.0; // of a CU
+        const double sets = std::floor(each / set), left = each - sets * set;
+        double t = sets * full;
+        if (left > 0)
+            t += sets > 0 ? 0.65 * alone + left * (full - 0.65 * alone) / set
+                          : alone + std::max(0.0, left - 1) * (full - alone) / (set - 1);
+        return t * count / n + (n > 1 ? 3 + join * blocks * n : 0);
+    };
+    long long splits = 1;
+    double best = 0.95 * time(1);
+    for (long long n = 2; n <= 64 && n * 4 <= count; n++)
+        if (time(n) < best)
+        {
+            best = time(n);
+            splits = n;
+        }
+    return splits;
+}
+
+} // namespace
+
 void kv_attention_deal(KvAttentionLaunch& p, int max_length)
 {
     const KvView& c = p.cache;
     const int group = p.group.d;
     const long long rows = static_cast<long long>(c.max_rows) * group;
+    // Each tile of 16 rows reads the keys for itself. 16 sequences of 8000 keys,
+    // 8 heads of 128 and as many rows (us), tiles of 16 and of 128:
+    //   bf16: 16 rows 99, 99; 32 rows 155, 100. One of 4000: 16 rows 15, 17.
+    //   four bits, which a tile of 128 unpacks into LDS: 16 rows 38, 90; 32 rows
+    //   60, 92; 48 rows 82, 96; 64 rows 108, 97.
     p.few = rows <= (p.four ? 3 : 1) * kRowTile;
     const int tile_rows = p.few ? kRowTile : kTileRows;
     p.tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
@@ -1304,13 +1360,17 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
         return k;
     };
     // Few workgroups at the end would have the card to themselves: lengths may
-    // differ, so parts are not longer than this.
+    // differ, so parts are not longer than this. One row each over 99 sequences of
+    // 2000 keys and one of 131072, 8 heads (us), parts of 16384, 8192 and 4096
+    // keys at most: 317, 305, 282 (450 unsplit); over 127 of 4096 beside a chunk of
+    // 1024 rows: 439, 441, 488; over 64 of 16384: 722, 719, 719.
     const long long least = (count + kLongPart - 1) / kLongPart;
     if (p.few)
     {
         // The split with the least time, in key tiles of a workgroup: rounds of
         // workgroups (two or three a CU, by their registers), each with its start
-        // and its part, and the join.
+        // and its part, and the join. (A join that counts half, twice or four times
+        // as much changes calls of 700 to 6000 keys by -1 to 7 us.)
         const long long blocks = static_cast<long long>(p.tiles) * c.heads * c.sequences;
         const long long slots = 256 * (p.four || p.head_dim == 64 ? 3 : 2);
         long long best = -1, splits = 1;
@@ -1329,34 +1389,43 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
         p.one = p.more = parts(splits);
         return;
     }
-    // Too few to fill the device: two a CU, with at least eight key tiles.
-    const auto fill = [&](long long blocks) {
-        return blocks < 192 ? std::min((511 + blocks) / blocks, count / 8) : 1;
+    // (Without a window the rows of a chunk see, on the average, all but half of it.)
+    const double average =
+        p.mask.window > 0 ? count : std::max(1.0, (keys - 0.5 * std::min<long long>(c.max_rows, keys)) / kKeyTile);
+    const auto fill = [&](long long blocks, long long block_rows) {
+        return tile_splits(p, blocks, std::min(block_rows, static_cast<long long>(kTileRows)), average);
     };
     if (p.tiles == 1)
     {
-        p.one = p.more = parts(std::max(least, fill(static_cast<long long>(c.heads) * c.sequences)));
+        p.one = p.more = parts(std::max(least, fill(static_cast<long long>(c.heads) * c.sequences, rows)));
         p.parts = p.one.splits;
         return;
     }
     // (A sequence's last row tile may have one row.)
     const long long most = std::min(static_cast<long long>(p.tiles) * c.sequences,
                                     static_cast<long long>(c.total_rows) * group / kTileRows + c.sequences);
-    p.more = parts(fill(c.heads * most));
-    // Single tokens and short chunks beside longer ones: if there can be any,
-    // they are dealt out by themselves.
+    p.more = parts(fill(c.heads * most, kTileRows));
     p.one = parts(1);
+    // Single tokens and short chunks beside longer ones, if there can be any, are
+    // dealt out by themselves; how many there are, and how long, is not known here,
+    // so either kind is split only if few workgroups are there for it.
     const int one_rows = kTileRows / group;
     if (one_rows > 0 && c.total_rows - (c.sequences - 1ll) * c.max_rows <= one_rows)
     {
-        p.one = parts(std::max(least, fill(c.heads * (c.sequences - 1ll))));
+        const auto few = [&](long long blocks) {
+            return blocks < 192 ? std::min((511 + blocks) / blocks, count / 8) : 1;
+        };
+        p.more = parts(few(c.heads * most));
+        p.one = parts(std::max(least, few(c.heads * (c.sequences - 1ll))));
         if (static_cast<long long>(one_rows) * c.sequences < c.total_rows)
         {
             p.one.seq_rows = one_rows;
             p.one.rows = static_cast<long long>(one_rows) * c.sequences;
         }
     }
-    // A workgroup without work takes about 0.8 ns of the launch, the list 4 us.
+    // A workgroup without work takes about 0.8 ns of the launch, the list 4 us: a
+    // chunk of 4096 rows beside 127 single tokens over 300 keys, 32/8 heads: 308
+    // us, listed 185; beside 511: 916 and 306; beside 7: 183 and 174.
     const long long each = std::max(static_cast<long long>(p.tiles) * p.more.splits, static_cast<long long>(p.one.splits));
     const long long listed = static_cast<long long>(c.total_rows) * group / kTileRows * p.more.splits +
                              static_cast<long long>(c.sequences) * std::max(p.one.splits, p.more.splits);

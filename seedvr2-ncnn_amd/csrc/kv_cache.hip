@@ -4,7 +4,8 @@
 // their slots and the queries where the attention reads them. Bound by memory:
 // a row is read once and written once. A workgroup takes the rows of a few
 // tokens; the (cos, sin) of a token's pairs are computed once and shared by its
-// heads.
+// heads. 13311 tokens of 20 heads of 128, queries, keys and values in bf16: 85 us,
+// 4.8 TB/s (a copy reaches 4.9); 16 tokens: 4.5 us, a launch.
 //
 // Angles: positions of a long session are far from zero, so an angle's turns
 // are a 64-bit fraction times the position, of which the whole turns fall off
@@ -436,7 +437,9 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvReadLaunch p,
 }
 
 // Tokens a workgroup and heads a part: whole tokens, four at a time, where
-// they fill the device, else a row a lane group.
+// they fill the device, else a row a lane group. 20 heads of 128, bf16 (us), one
+// token and four: 512 tokens 9.6, 11; 1024 10, 13; 2048 17, 16; 6000 39, 32; in
+// four bits 14, 20; 18, 22; 28, 27; 65, 46.
 struct Deal
 {
     bool four_tokens;
