@@ -1217,76 +1217,100 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
 }
 
 // Joins the parts of a row: M = max m_i, out = sum 2^(m_i - M) o_i / sum
-// 2^(m_i - M) l_i, in the parts' order; parts without a key are left out. One
-// wave a row and query head at a time. Bound by latency: all parts' maxima and
-// sums come with one load, their rows with independent ones, eight at a time.
-// 3.2 us for 20 rows, 3.6 us for 2048.
-template <int D, bool F32>
+// 2^(m_i - M) l_i, in an order that the number of parts gives; parts without a
+// key are left out. 16 lanes hold a row: with GROUPS 1 a wave takes four rows of
+// at most 16 parts, with 4 it takes the parts of one, at most 64, in four. All
+// parts' maxima and sums come with one load, their rows with independent ones,
+// eight at a time.
+// MERGE
+template <int D, bool F32, int GROUPS>
 __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p)
 {
-    constexpr int kPer = D / 64;
+    constexpr int kPer = D / 16;      // features a lane
+    constexpr int kRows = 4 / GROUPS; // rows of a wave
     constexpr int kBatch = 8;
-    const KvView& c = p.cache;
-    const KvSequence s = kv_sequence(c, blockIdx.y);
+    const KvSequence s = kv_sequence(p.cache, blockIdx.y);
     const KvParts k = !p.few && s.rows * p.group.d > kTileRows ? p.more : p.one;
     if (k.splits == 1)
         return;
-    const int lane = threadIdx.x & 63;
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < s.rows * p.heads.d; i += gridDim.x * 4)
+    const int lane = threadIdx.x & 15;
+    const int group = (threadIdx.x >> 4) & 3;
+    const int first_part = GROUPS == 1 ? 0 : group;
+    const int rows = s.rows * p.heads.d;
+    for (int i0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows; i0 < rows; i0 += gridDim.x * 4 * kRows)
     {
+        // (Past the last row: that one again, not stored.)
+        const int i = min(i0 + (GROUPS == 1 ? group : 0), rows - 1);
         const int token = kv_divide(i, p.heads);
         const int head = i - token * p.heads.d;
         const size_t row = part_index(k, blockIdx.y, s, token);
-        const float2 mine = lane < k.splits ? *reinterpret_cast<const float2*>(part_stats(p, k, D, lane, row, head))
-                                            : make_float2(-INFINITY, 0.f);
+        const int mine_part = lane * GROUPS + first_part;
+        const float2 mine = mine_part < k.splits
+                                ? *reinterpret_cast<const float2*>(part_stats(p, k, D, mine_part, row, head))
+                                : make_float2(-INFINITY, 0.f);
         float m = mine.x;
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1)
+        for (int off = 1; off < 16 * GROUPS; off *= 2)
             m = fmaxf(m, __shfl_xor(m, off, 64));
-        const bool there = mine.x != -INFINITY;
-        const float weight = there ? __builtin_amdgcn_exp2f(mine.x - (m == -INFINITY ? 0.f : m)) : 0.f;
-        float sum = there ? weight * mine.y : 0.f;
+        const bool has_keys = mine.x != -INFINITY;
+        // (< 0: no keys.)
+        const float weight = has_keys ? __builtin_amdgcn_exp2f(mine.x - m) : -1.f;
+        float sum = has_keys ? weight * mine.y : 0.f;
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1)
+        for (int off = 1; off < 16 * GROUPS; off *= 2)
             sum += __shfl_xor(sum, off, 64);
-        unsigned long long left = __ballot(there);
         float v[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; e++)
             v[e] = 0.f;
-        while (left)
+#pragma unroll 1
+        for (int t = 0; t < 16 && t * GROUPS < k.splits; t += kBatch)
         {
-            float part[kBatch][kPer], by[kBatch];
+            float4 part[kBatch][kPer / 4];
+            float by[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; b++)
             {
-                // (Past the last part: that one again, with no weight.)
-                const int j = __builtin_amdgcn_readfirstlane(left ? __ffsll(left) - 1 : 0);
-                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j));
-                const float* const src = part_row(p, k, D, j, row, head) + lane * kPer;
-                by[b] = left ? w : 0.f;
+                by[b] = __shfl(weight, t + b, 16);
+                const bool there = !(by[b] < 0.f);
+                const float4* const src = reinterpret_cast<const float4*>(
+                    part_row(p, k, D, (t + b) * GROUPS + first_part, row, head) + lane * kPer);
 #pragma unroll
-                for (int e = 0; e < kPer; e++)
-                    part[b][e] = left ? src[e] : 0.f;
-                left &= left - 1;
+                for (int e = 0; e < kPer / 4; e++)
+                    part[b][e] = there ? src[e] : make_float4(0.f, 0.f, 0.f, 0.f);
+                by[b] = there ? by[b] : 0.f;
             }
 #pragma unroll
             for (int b = 0; b < kBatch; b++)
 #pragma unroll
-                for (int e = 0; e < kPer; e++)
-                    v[e] = fmaf(by[b], part[b][e], v[e]);
+                for (int e = 0; e < kPer / 4; e++)
+                {
+                    v[4 * e] = fmaf(by[b], part[b][e].x, v[4 * e]);
+                    v[4 * e + 1] = fmaf(by[b], part[b][e].y, v[4 * e + 1]);
+                    v[4 * e + 2] = fmaf(by[b], part[b][e].z, v[4 * e + 2]);
+                    v[4 * e + 3] = fmaf(by[b], part[b][e].w, v[4 * e + 3]);
+                }
         }
+        if (GROUPS > 1)
+#pragma unroll
+            for (int e = 0; e < kPer; e++)
+            {
+                v[e] += __shfl_xor(v[e], 16, 64);
+                v[e] += __shfl_xor(v[e], 32, 64);
+            }
+        if (GROUPS > 1 ? group != 0 : i0 + group >= rows)
+            continue;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         unsigned char* const dst = const_cast<unsigned char*>(p.out.data) +
                                    static_cast<long long>(s.first + token) * p.out.stride +
-                                   static_cast<long long>(head) * D * (F32 ? 4 : 2);
+                                   (static_cast<long long>(head) * D + lane * kPer) * (F32 ? 4 : 2);
 #pragma unroll
-        for (int e = 0; e < kPer; e++)
+        for (int e = 0; e < kPer; e += 4)
         {
             if (F32)
-                reinterpret_cast<float*>(dst)[lane * kPer + e] = v[e] * inv;
+                store4(reinterpret_cast<float*>(dst) + e, v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv);
             else
-                reinterpret_cast<__bf16*>(dst)[lane * kPer + e] = static_cast<__bf16>(v[e] * inv);
+                store4(reinterpret_cast<uint16_t*>(dst) + e, v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv);
         }
     }
 }
@@ -1441,13 +1465,25 @@ TileDeal tile_deal(const KvAttentionLaunch& p)
     return tile_deal(p.cache.heads * (p.listed ? 1 : p.cache.sequences), static_cast<int>(p.parts));
 }
 
-// Workgroups of the join of a sequence's rows: one for four of them in a small
-// call, for many sequences no more than a single token needs.
-int merge_blocks(const KvAttentionLaunch& p)
+// The join of a sequence's rows: whether a wave takes one of them, for few rows
+// and for many parts, and its workgroups, for many sequences no more than a
+// single token needs.
+struct MergeDeal
 {
-    const long long rows = p.more.splits > 1 ? p.cache.max_rows : std::min(p.cache.max_rows, kTileRows / p.group.d);
-    return static_cast<int>(std::min((rows * p.heads.d + 3) / 4,
-                                     std::max((p.heads.d + 3ll) / 4, 8192ll / p.cache.sequences)));
+    bool one_row;
+    int blocks;
+};
+
+MergeDeal merge_deal(const KvAttentionLaunch& p)
+{
+    const long long tokens = p.more.splits > 1 ? p.cache.max_rows : std::min(p.cache.max_rows, kTileRows / p.group.d);
+    MergeDeal d;
+    d.one_row = tokens * p.heads.d * p.cache.sequences < 8192 ||
+                std::max(p.one.splits, p.more.splits) > 16;
+    const int each = d.one_row ? 4 : 16; // rows of a workgroup
+    d.blocks = static_cast<int>(std::min((tokens * p.heads.d + each - 1) / each,
+                                         std::max((p.heads.d + each - 1ll) / each, 8192ll / p.cache.sequences)));
+    return d;
 }
 
 size_t partial_floats(const KvAttentionLaunch& p, const KvParts& k)
@@ -1514,8 +1550,12 @@ hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || (p.one.splits == 1 && p.more.splits == 1))
         return e;
-    hipLaunchKernelGGL((kv_merge_kernel<D, F32>), dim3(merge_blocks(p), p.cache.sequences),
-                       dim3(256), 0, stream, p);
+    const MergeDeal m = merge_deal(p);
+    const dim3 grid(m.blocks, p.cache.sequences);
+    if (m.one_row)
+        hipLaunchKernelGGL((kv_merge_kernel<D, F32, 4>), grid, dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((kv_merge_kernel<D, F32, 1>), grid, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 
