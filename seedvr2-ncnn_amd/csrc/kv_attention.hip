@@ -697,20 +697,20 @@ __global__ __launch_bounds__(kListThreads) void kv_list_kernel(const KvAttention
 }
 
 // A tile of 128 rows, 32 a wave; key tiles of 32 go through LDS, which all
-// waves read. Bound by the matrix cores, and next by what feeds them: an operand
-// read from LDS serves one MFMA, so that MFMAs at full rate take all of LDS's
-// bandwidth. Three workgroups share a CU (two of fp32 rows, whose queries take
-// three times the registers), so that one's softmax, waits and edges run beside
-// the others' products: nothing else of the loop overlaps by itself, and
-// schedules within a wave gained less. 16384 rows of 20 heads, 128 features,
-// causal: 1300 us so (1.04 PFLOP/s; a matrix product of 8192^3 reaches 1.2), the
-// matrix cores and the vector units busy for half of it each. Two workgroups that
+// waves read. Bound by the matrix cores, next to them by the softmax's vector
+// instructions, and by power: the clock falls to about 1.75 GHz. Three workgroups
+// share a CU (two of fp32 rows, whose queries take three times the registers), so
+// that one's softmax, waits and edges run beside the others' products: nothing
+// else of the loop overlaps by itself, and schedules within a wave gained less.
+// 16384 rows of 20 heads, 128 features, causal: 1300 us so (1.04 PFLOP/s; a matrix
+// product of 8192^3 reaches 1.2), the matrix cores and the vector units busy for
+// somewhat more than half of it each, LDS for a third. Two workgroups that
 // take the scores of the next block beside a block's softmax: 1440 us; one such
 // of eight waves, whose barriers keep them in step: 1557; four waves of 64 rows,
 // which read half the operands but leave a matrix core one wave to be fed by:
 // 1834. Without its loads of keys and values the loop would take 1183 us, without
-// the exponentials 1244, without half of its LDS reads 1270: no single part
-// bounds it.
+// the exponentials 1244, without half of its LDS reads 1270, with bank conflicts
+// that double the LDS cycles 1318: no single part bounds it.
 //
 // S^T = K Q^T (32x32x16): lane (col = lane % 32, half = lane / 32) holds row
 // col's scores of keys 8 (i / 4) + 4 half + i % 4, i < 16; eight of them in a row
@@ -880,7 +880,7 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     };
 
     // Where a 16-byte chunk of a row lies in LDS: chunks are permuted so that
-    // both operands' reads touch all banks (K: 16 rows, one chunk each; V: four
+    // both operands' reads touch all 64 banks (K: 16 rows, one chunk each; V: four
     // rows, two chunks each).
     auto k_chunk = [](int r, int chunk) { return chunk ^ (D == 128 ? r & 15 : (r >> 1) & 7); };
     auto v_chunk = [](int r, int chunk) { return chunk ^ (D == 128 ? (r & 3) << 2 : (r & 2) << 1); };
@@ -1222,7 +1222,9 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
 // at most 16 parts, with 4 it takes the parts of one, at most 64, in four. All
 // parts' maxima and sums come with one load, their rows with independent ones,
 // eight at a time.
-// MERGE
+// Bound by latency where rows are few: 20 rows of 6 parts 4.4 us, of 64 parts 6.2
+// (a wave a row, eight parts at a time: 4.2 and 8.8); by memory where they are
+// many: 28160 rows of three parts 13.1 us, 4.5 TB/s (a wave a row 18.8).
 template <int D, bool F32, int GROUPS>
 __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p)
 {
