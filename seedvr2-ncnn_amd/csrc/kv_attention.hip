@@ -130,6 +130,13 @@ __device__ __forceinline__ float* part_stats(const KvAttentionLaunch& p, const K
     return k.partial + k.splits * all * dim + (part * all + row * p.heads.d + head) * 2;
 }
 
+// Whether some row of those from `first` to `last` (spans) may see some key of the
+// 16 from `key` on.
+__device__ __forceinline__ bool some_row_sees(int key, const KvSpan& first, const KvSpan& last)
+{
+    return key < last.end && (key + 16 > first.begin || key < last.sinks);
+}
+
 // One row tile of 16 rows, one part of its keys: each wave takes every fourth
 // key tile (32 keys) by itself, with K from memory straight into the MFMA
 // operand registers and V through the wave's own LDS, from which it is read
@@ -256,7 +263,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
             const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
             if (ok && key < span_last.end)
                 t.there |= 1u << b;
-            if (!ok)
+            // (A page that the tile has no visible key in is not needed.)
+            if (!ok && some_row_sees(key, span_first, span_last))
                 bad = AWA_KV_BAD_PAGE;
             t.base[b] = static_cast<unsigned>(__builtin_amdgcn_readfirstlane(
                 (((ok ? page : 0) * c.heads + head) << c.page_shift) + (key & slot_mask)));
@@ -1073,10 +1081,10 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     // (LDS alone: the loads of the next tile go on.)
     auto wait_lds = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // The first keys of this tile and the next, the next one's pages, and which
-    // blocks of this tile (and of any) have none.
+    // blocks of this tile have none.
     int key_now = 0, key_next = 0;
     Pages pages_next{};
-    unsigned none = 0, bad = 0;
+    unsigned none = 0;
     if (t_begin < t_end)
     {
         if (tid == 0)
@@ -1109,7 +1117,6 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
             load_four(row_next);
         else
             load(row_next, 1 - slot);
-        bad |= none;
         const int key_third = tile_key(t + 2);
         pages_next = pages_of(key_third);
         bool edge = false;
@@ -1120,6 +1127,11 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
         {
             edge = none != 0u || !((key_now >= w_last.begin && key_now + kKeys <= w_first.end) ||
                                    key_now + kKeys <= w_first.sinks);
+            // (A page that the tile has no visible key in is not needed.)
+            if (((none & 1u) && some_row_sees(key_now, first, last)) ||
+                ((none & 2u) && some_row_sees(key_now + 16, first, last)))
+                if (c.status && tid == 0)
+                    atomicOr(c.status, AWA_KV_BAD_PAGE);
             uint4* const v = reinterpret_cast<uint4*>(v_tile);
             constexpr int kMine = kKeys * kRowChunks / kThreads;
             bool fine = true;
@@ -1190,8 +1202,6 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
     }
     // No load of this wave may be on its way into LDS when it ends.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (bad && c.status && tid == 0)
-        atomicOr(c.status, AWA_KV_BAD_PAGE);
     const float sum = sum_xor32(row_sum);
     if (wave_row0 + col >= rows)
         return;

@@ -578,6 +578,28 @@ def test_no_visible_key_gives_zeros(gpu):
         assert cache.status() == A.KV_BAD_PAGE
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "4bit"])
+@pytest.mark.parametrize("count", [1, 40, 300])
+def test_pages_that_no_row_sees_may_be_given_back(gpu, fmt, count):
+    """Table entries between the first slots and the window name no page: they
+    are not needed, also where a visible slot is next to theirs."""
+    rng = np.random.default_rng(48)
+    for length, window, sinks in ((700, 50, 5), (701, 47, 0), (716, 64, 17), (690, 33, 40)):
+        cache = M.Cache(fmt, [length], 2, 64, 16)
+        seen = np.zeros(length, bool)
+        for j in range(count):
+            seen |= M.visible(length - count + j, length, window, sinks, 1)
+        for page in range(cache.width):
+            if not seen[16 * page:16 * page + 16].any():
+                cache.table[0, page] = -1
+        assert (cache.table < 0).any()
+        cache.upload()
+        q = new_rows(rng, [count], 4, 64, "bf16")
+        got = run_attention(cache, [count], q, "bf16", window, sinks)
+        check_attention(cache, [count], q, "bf16", got, window, sinks)
+        assert cache.status() == 0
+
+
 def test_same_bits_every_time_and_on_another_stream(gpu):
     rng = np.random.default_rng(25)
     for counts, lengths in ([1, 1], [3000, 800]), ([200, 3], [900, 1200]):
@@ -732,5 +754,61 @@ def test_captured_step_follows_the_lengths(gpu):
             want, bound = M.attention(replayed["qo"][j:j + 1], k, v, int(cache.lengths[j]), 0, 4, 1, 128 ** -0.5,
                                       "bf16")
             assert (np.abs(replayed["out"][j:j + 1] - want) <= bound).all()
+    assert rt.hipGraphExecDestroy(run) == 0 and rt.hipGraphDestroy(graph) == 0
+    stream.destroy()
+
+
+def test_captured_mixed_call_follows_its_rows(gpu):
+    """One graph of an attention over many sequences, replayed while which of
+    them has the chunk, and how long they are, changes; an eager call of the same
+    between the replays."""
+    rng = np.random.default_rng(32)
+    n, most, heads, dim = 400, 600, 8, 64
+    cache = M.Cache("bf16", [most + 100] * n, 4, dim, 32)
+    desc = cache.upload()
+    total = most + n - 1 + 5  # rows behind the last sequence among them
+    q, out = M.Rows(np.zeros((total, heads, dim)), "bf16"), M.Rows(np.zeros((total, heads, dim)), "bf16")
+    cu = M.ints(np.zeros(n + 1))
+    rows, mask = A.KvRows(most, cu.ptr), A.KvMask(0, 0, 1, most + 100)
+    need = A.kv_attention_workspace(desc, rows, q.blob, mask)
+    assert need > 0  # the parts' numbers among it
+    ws, other = A.DeviceBuffer(max(need, 16)), A.DeviceBuffer(max(need, 16))
+    stream, rt = A.Stream(), hip()
+
+    def step(workspace):
+        A.kv_attention(desc, rows, q.blob, mask, dim ** -0.5, out.blob, workspace.ptr, need, stream)
+
+    def set_rows(i):
+        counts = [1] * n
+        counts[(7 + 41 * i) % n] = most - 50 * i
+        counts[(20 + 3 * i) % n] = 0
+        cu.upload(np.cumsum([0] + counts).astype(np.int32))
+        cache.set(lengths=[c + int(x) for c, x in zip(counts, rng.integers(0, 100, n))])
+        return counts
+
+    set_rows(0)
+    step(ws)
+    stream.synchronize()
+    s, graph, run = ctypes.c_void_p(stream.handle), ctypes.c_void_p(), ctypes.c_void_p()
+    assert rt.hipStreamBeginCapture(s, 2) == 0
+    step(ws)
+    assert rt.hipStreamEndCapture(s, ctypes.byref(graph)) == 0
+    assert rt.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0) == 0
+    for i in range(1, 4):
+        counts = set_rows(i)
+        x = new_rows(rng, [total], heads, dim, "bf16", std=2.0)
+        q.buf.upload(A.f32_to_bf16_bits(x))
+        out.buf.upload(A.f32_to_bf16_bits(np.full(x.shape, 5.0, np.float32)))
+        A.synchronize()
+        assert rt.hipGraphLaunch(run, s) == 0
+        stream.synchronize()
+        replayed = out.read()
+        assert (replayed[sum(counts):] == 5.0).all()
+        out.buf.zero()
+        A.synchronize()
+        step(other)
+        stream.synchronize()
+        np.testing.assert_array_equal(out.read()[:sum(counts)], replayed[:sum(counts)])
+        check_attention(cache, counts, x, "bf16", replayed)
     assert rt.hipGraphExecDestroy(run) == 0 and rt.hipGraphDestroy(graph) == 0
     stream.destroy()
