@@ -90,9 +90,30 @@ __device__ __forceinline__ int find_sequence(const KvView& c, int t)
     if (!c.cu)
         return t / c.max_rows;
     const int lane = threadIdx.x & 63;
+    // (One with more rows than there may be takes no part.)
+    const auto has = [&](int s) {
+        const int from = c.cu[s], to = c.cu[s + 1];
+        return from >= 0 && from <= t && t < to && to - from <= c.max_rows;
+    };
+    // The first that ends behind t, in 64ths of what is left; with cu_rows in
+    // order it has t.
+    if (c.sequences > 64)
+    {
+        int step = 1, s = 0;
+        while (step * 64 < c.sequences)
+            step *= 64;
+        for (; step > 0; step /= 64)
+        {
+            const int at = s + (lane + 1) * step;
+            const unsigned long long not_yet = __ballot(at <= c.sequences && c.cu[min(at, c.sequences)] <= t);
+            s += (not_yet == ~0ull ? 64 : __ffsll(~not_yet) - 1) * step;
+        }
+        if (s < c.sequences && has(s))
+            return s;
+    }
     for (int i = 0; i < c.sequences; i += 64)
     {
-        const bool in = i + lane < c.sequences && c.cu[i + lane] <= t && t < c.cu[i + lane + 1];
+        const bool in = i + lane < c.sequences && has(i + lane);
         const unsigned long long found = __ballot(in);
         if (found)
             return i + __ffsll(found) - 1;

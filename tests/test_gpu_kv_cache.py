@@ -275,6 +275,34 @@ def test_many_rows_and_sequences(gpu):
         assert (ko.read()[at:] == 5.0).all()
 
 
+@pytest.mark.parametrize("n", [65, 4097])
+@pytest.mark.parametrize("order", ["kept", "broken"])
+def test_rows_of_thousands_of_sequences(gpu, n, order):
+    """Every row finds its sequence, beside empty ones; of cu_rows out of order all
+    rows that one sequence alone claims."""
+    rng = np.random.default_rng(12)
+    counts = [int(c) for c in rng.choice([0, 1, 1, 1, 2], n)]
+    cu = np.cumsum([0] + counts)
+    total = int(cu[-1]) + 3
+    if order == "broken":
+        cu[n // 2] = 0  # one sequence ends before it begins, the next has too many rows
+    cache = M.Cache("bf16", [c + 1 for c in counts], 1, 64, 16)
+    desc = cache.upload()
+    x = new_rows(rng, [total], 1, 64, "bf16")
+    A.kv_append(desc, A.KvRows(2, M_keep(cu)), M.Rows(x, "bf16").blob, M.Rows(x, "bf16").blob)
+    A.synchronize()
+    assert cache.status() == (A.KV_BAD_ROWS if order == "broken" else 0)
+    want = cache.host["v"].copy()
+    for s in range(n):
+        rows = int(cu[s + 1]) - int(cu[s])
+        if not 0 <= rows <= 2:
+            continue
+        for j in range(rows):
+            slot = int(cache.lengths[s]) - rows + j
+            want[cache.table[s, slot // 16], 0, slot % 16] = A.f32_to_bf16_bits(x[cu[s] + j, 0])
+    np.testing.assert_array_equal(cache.download()["v"], want)
+
+
 def test_what_does_not_fit_is_left_out_and_told(gpu):
     """Bad pages, lengths and rows: told in the status, nothing read or written for them."""
     rng = np.random.default_rng(9)
