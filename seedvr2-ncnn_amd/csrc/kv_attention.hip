@@ -664,7 +664,10 @@ __global__ __launch_bounds__(kListThreads) void kv_list_kernel(const KvAttention
             const int rows = s.rows * p.group.d;
             bad |= s.bad;
             if (rows > kTileRows)
-                n[0] = static_cast<long long>((rows + kTileRows - 1) / kTileRows) * p.more.splits;
+            {
+                const int tiles = (rows + kTileRows - 1) / kTileRows, split = min(tiles, p.more.tiles);
+                n[0] = tiles - split + static_cast<long long>(split) * p.more.splits;
+            }
             else if (rows > 0)
                 n[1] = p.one.splits;
         }
@@ -775,13 +778,16 @@ __global__ __launch_bounds__(256, F32 ? 2 : 3) void kv_tile_kernel(const KvAtten
         atomicOr(c.status, static_cast<int>(s.bad));
     const int rows = s.rows * p.group.d;
     const bool one = rows <= kRows;
-    const int splits = one ? p.one.splits : p.more.splits;
     const int part_tiles = one ? p.one.part_tiles : p.more.part_tiles;
-    const int split = item.part % splits;
-    // (Tiles from the end, which see the most keys; unless listed, those of all
-    // sequences in step, so that the longest sequence's come first.)
+    // Row tiles from the end, which see the most keys; unless listed, those of all
+    // sequences in step, so that the longest sequence's come first. The first of
+    // a sequence, which come last, may alone be split.
     const int tiles_all = one ? 1 : p.listed ? (rows + kRows - 1) / kRows : p.tiles;
-    const int tile = tiles_all - 1 - item.part / splits;
+    const int whole = one ? 0 : max(tiles_all - p.more.tiles, 0);
+    const int splits = item.part < whole ? 1 : one ? p.one.splits : p.more.splits;
+    const int part = item.part < whole ? item.part : item.part - whole;
+    const int tile = (item.part < whole ? tiles_all : tiles_all - whole) - 1 - part / splits;
+    const int split = part % splits;
     const int row0 = tile * kRows;
     if (tile < 0 || row0 >= rows)
         return;
@@ -1242,19 +1248,24 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
     constexpr int kRows = 4 / GROUPS; // rows of a wave
     constexpr int kBatch = 8;
     const KvSequence s = kv_sequence(p.cache, blockIdx.y);
-    const KvParts k = !p.few && s.rows * p.group.d > kTileRows ? p.more : p.one;
+    const bool more = !p.few && s.rows * p.group.d > kTileRows;
+    const KvParts k = more ? p.more : p.one;
     if (k.splits == 1)
         return;
     const int lane = threadIdx.x & 15;
     const int group = (threadIdx.x >> 4) & 3;
     const int first_part = GROUPS == 1 ? 0 : group;
-    const int rows = s.rows * p.heads.d;
+    // (Rows of tiles that are not split are there already.)
+    const int split_rows = more ? p.more.tiles * kTileRows : kTileRows;
+    const int rows = min(s.rows, kv_divide(split_rows - 1, p.group) + 1) * p.heads.d;
     for (int i0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows; i0 < rows; i0 += gridDim.x * 4 * kRows)
     {
         // (Past the last row: that one again, not stored.)
         const int i = min(i0 + (GROUPS == 1 ? group : 0), rows - 1);
         const int token = kv_divide(i, p.heads);
         const int head = i - token * p.heads.d;
+        if (token * p.group.d + head - kv_divide(head, p.group) * p.group.d >= split_rows)
+            continue;
         const size_t row = part_index(k, blockIdx.y, s, token);
         const int mine_part = lane * GROUPS + first_part;
         const float2 mine = mine_part < k.splits
@@ -1332,39 +1343,92 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(const KvAttentionLaunch p
 namespace
 {
 
-// Parts of a row tile of 128 rows with the least time for `blocks` of them, which
-// see `count` key tiles on the average. Measured, in us a key tile: a workgroup that
-// has a CU to itself, and a CU's full set of them side by side (which a CU takes
-// set after set; of the last one it has a part); a part's rows are written and
-// read again. 8 heads of 128 over 8000 keys (us): 8 workgroups 198, split 28;
-// 64 (1024 rows) 191, split 58. 20 heads: 220 (1408 rows over 31408 keys) 728, in
-// three parts 504; 320 (2048 over 8048) 218, in two 204; 460 265, in two 322; 100
-// (640 over 640) 26, in two 31.
-long long tile_splits(const KvAttentionLaunch& p, long long blocks, long long block_rows, double count)
+// What workgroups of kv_tile_kernel take, measured, in us.
+struct TileTimes
 {
-    const bool half = p.head_dim == 64;
-    const double alone = (p.f32 ? 1.35 : p.four ? 1.0 : 0.75) * (half ? 0.85 : 1.0);
-    const double full = (p.f32 ? 1.8 : p.four ? 1.7 : 1.55) * (half ? 0.9 : 1.0);
-    const int set = p.f32 ? (half && !p.four ? 3 : 2) : half ? 4 : 3;
-    const double join = 0.045 * block_rows / kTileRows * p.head_dim / 128;
+    double alone; // a key tile, of one that has a CU to itself
+    double full;  // of a CU's full set of them side by side
+    int set;      // in a full set
+    double join;  // writing and reading a part again
+
+    TileTimes(const KvAttentionLaunch& p, long long block_rows)
+    {
+        const bool half = p.head_dim == 64;
+        alone = (p.f32 ? 1.35 : p.four ? 1.0 : 0.75) * (half ? 0.85 : 1.0);
+        full = (p.f32 ? 1.8 : p.four ? 1.7 : 1.55) * (half ? 0.9 : 1.0);
+        set = p.f32 ? (half && !p.four ? 3 : 2) : half ? 4 : 3;
+        join = 0.045 * std::min(block_rows, static_cast<long long>(kTileRows)) / kTileRows * p.head_dim / 128;
+    }
+};
+
+struct Split
+{
+    long long n;
+    double time;
+};
+
+// Parts of a row tile of 128 rows with the least time for `blocks` of them, which
+// see `count` key tiles on the average: a CU takes one full set of workgroups
+// after the other, and of the last one it has a part. 8 heads of 128 over 8000
+// keys (us): 8 workgroups 198, split 28; 64 (1024 rows) 191, split 58. 20 heads:
+// 220 (1408 rows over 31408 keys) 728, in three parts 504; 320 (2048 over 8048)
+// 218, in two 204; 460 265, in two 322; 100 (640 over 640) 26, in two 31.
+Split tile_splits(const TileTimes& c, long long blocks, double count)
+{
     const auto time = [&](long long n) {
         const double each = blocks * n / 256.0; // of a CU
-        const double sets = std::floor(each / set), left = each - sets * set;
-        double t = sets * full;
+        const double sets = std::floor(each / c.set), left = each - sets * c.set;
+        double t = sets * c.full;
         if (left > 0)
-            t += sets > 0 ? 0.65 * alone + left * (full - 0.65 * alone) / set
-                          : alone + std::max(0.0, left - 1) * (full - alone) / (set - 1);
-        return t * count / n + (n > 1 ? 3 + join * blocks * n : 0);
+            t += sets > 0 ? 0.65 * c.alone + left * (c.full - 0.65 * c.alone) / c.set
+                          : c.alone + std::max(0.0, left - 1) * (c.full - c.alone) / (c.set - 1);
+        return t * count / n + (n > 1 ? 3 + c.join * blocks * n : 0);
     };
-    long long splits = 1;
-    double best = 0.95 * time(1);
+    Split s{1, time(1)};
+    double best = 0.95 * s.time;
     for (long long n = 2; n <= 64 && n * 4 <= count; n++)
         if (time(n) < best)
         {
             best = time(n);
-            splits = n;
+            s = {n, best};
         }
-    return splits;
+    return s;
+}
+
+// The same where only the first `tiles` row tiles of each of `units` are split,
+// which start last: the others fill whole sets, and the parts of these what is
+// left. n 1: none takes less time than `best`. 20 heads of 128 (us, without and
+// with): 5000 rows over 11000 keys 516, 433; 5760 over 11760 keys of four bits 721,
+// 547; 32/8 heads, 3500 over 15500: 869, 751.
+struct FirstSplit
+{
+    long long n;
+    int tiles;
+};
+
+FirstSplit first_splits(const TileTimes& c, long long blocks, long long units, int tiles, double count, double best)
+{
+    FirstSplit s{1, 0};
+    best *= 0.95;
+    const long long places = 256ll * c.set;
+    for (long long sets = std::max(1ll, blocks / places - 1); sets * places < blocks && sets <= blocks / places; sets++)
+    {
+        const long long first = (blocks - sets * places + units - 1) / units;
+        if (first >= tiles)
+            continue;
+        const double left = static_cast<double>(blocks - sets * places) / places;
+        for (long long n = 2; n <= 12 && n * 4 <= count; n++)
+        {
+            const double time =
+                ((sets + left) * c.full + 0.5 * c.alone / n) * count + 3 + c.join * units * first * n;
+            if (time < best)
+            {
+                best = time;
+                s = {n, static_cast<int>(first)};
+            }
+        }
+    }
+    return s;
 }
 
 } // namespace
@@ -1392,6 +1456,7 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
         KvParts k{};
         k.splits = static_cast<int>(std::max(1ll, std::min({splits, count, 64ll})));
         k.part_tiles = static_cast<int>((count + k.splits - 1) / k.splits);
+        k.tiles = p.tiles;
         k.rows = c.total_rows;
         return k;
     };
@@ -1404,11 +1469,11 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
     if (p.few)
     {
         // The split with the least time, in key tiles of a workgroup: rounds of
-        // workgroups (two or three a CU, by their registers), each with its start
+        // workgroups (two to four a CU, by their registers), each with its start
         // and its part, and the join. (A join that counts half, twice or four times
         // as much changes calls of 700 to 6000 keys by -1 to 7 us.)
         const long long blocks = static_cast<long long>(p.tiles) * c.heads * c.sequences;
-        const long long slots = 256 * (p.four || p.head_dim == 64 ? 3 : 2);
+        const long long slots = 256 * (p.head_dim == 64 ? 4 : p.four ? 3 : 2);
         long long best = -1, splits = 1;
         for (long long n = std::min(least, 64ll); n <= 64 && n <= count; n++)
         {
@@ -1428,19 +1493,40 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
     // (Without a window the rows of a chunk see, on the average, all but half of it.)
     const double average =
         p.mask.window > 0 ? count : std::max(1.0, (keys - 0.5 * std::min<long long>(c.max_rows, keys)) / kKeyTile);
-    const auto fill = [&](long long blocks, long long block_rows) {
-        return tile_splits(p, blocks, std::min(block_rows, static_cast<long long>(kTileRows)), average);
-    };
+    const TileTimes times(p, rows);
     if (p.tiles == 1)
     {
-        p.one = p.more = parts(std::max(least, fill(static_cast<long long>(c.heads) * c.sequences, rows)));
+        const Split split = tile_splits(times, static_cast<long long>(c.heads) * c.sequences, average);
+        p.one = p.more = parts(std::max(least, split.n));
         p.parts = p.one.splits;
         return;
     }
     // (A sequence's last row tile may have one row.)
     const long long most = std::min(static_cast<long long>(p.tiles) * c.sequences,
                                     static_cast<long long>(c.total_rows) * group / kTileRows + c.sequences);
-    p.more = parts(fill(c.heads * most, kTileRows));
+    const Split split = tile_splits(times, c.heads * most, average);
+    p.more = parts(split.n);
+    // Where all row tiles see about as many keys, the last ones alone may be split.
+    const long long fewest = std::max(1ll, std::min(keys, max_length - static_cast<long long>(c.max_rows)));
+    if (split.n == 1 && 2 * fewest > keys)
+    {
+        const FirstSplit first = first_splits(times, c.heads * most, static_cast<long long>(c.heads) * c.sequences,
+                                              p.tiles, average, split.time);
+        if (first.n > 1)
+        {
+            const long long tokens = (static_cast<long long>(first.tiles) * kTileRows + group - 1) / group;
+            p.more = parts(first.n);
+            p.more.tiles = first.tiles;
+            // (Of the last of them.)
+            const long long last = std::min(count, ((fewest + tokens) >> kKeyShift) + 2);
+            p.more.part_tiles = static_cast<int>((last + first.n - 1) / first.n);
+            if (tokens * c.sequences < c.total_rows)
+            {
+                p.more.seq_rows = static_cast<int>(tokens);
+                p.more.rows = tokens * c.sequences;
+            }
+        }
+    }
     p.one = parts(1);
     // Single tokens and short chunks beside longer ones, if there can be any, are
     // dealt out by themselves; how many there are, and how long, is not known here,
@@ -1462,7 +1548,8 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
     // A workgroup without work takes about 0.8 ns of the launch, the list 4 us: a
     // chunk of 4096 rows beside 127 single tokens over 300 keys, 32/8 heads: 308
     // us, listed 185; beside 511: 916 and 306; beside 7: 183 and 174.
-    const long long each = std::max(static_cast<long long>(p.tiles) * p.more.splits, static_cast<long long>(p.one.splits));
+    const long long each = std::max(p.tiles - p.more.tiles + static_cast<long long>(p.more.tiles) * p.more.splits,
+                                    static_cast<long long>(p.one.splits));
     const long long listed = static_cast<long long>(c.total_rows) * group / kTileRows * p.more.splits +
                              static_cast<long long>(c.sequences) * std::max(p.one.splits, p.more.splits);
     p.listed = (each * c.sequences - listed) * c.heads > 10000;
@@ -1488,7 +1575,9 @@ struct MergeDeal
 
 MergeDeal merge_deal(const KvAttentionLaunch& p)
 {
-    const long long tokens = p.more.splits > 1 ? p.cache.max_rows : std::min(p.cache.max_rows, kTileRows / p.group.d);
+    const long long first = (static_cast<long long>(p.more.tiles) * kTileRows + p.group.d - 1) / p.group.d;
+    const long long tokens = std::min(static_cast<long long>(p.cache.max_rows),
+                                      p.more.splits > 1 ? first : kTileRows / p.group.d);
     MergeDeal d;
     d.one_row = tokens * p.heads.d * p.cache.sequences < 8192 ||
                 std::max(p.one.splits, p.more.splits) > 16;

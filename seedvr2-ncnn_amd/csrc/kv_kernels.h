@@ -177,6 +177,7 @@ hipError_t launch_kv_read(const KvReadLaunch& p, hipStream_t stream);
 struct KvParts
 {
     int splits, part_tiles;
+    int tiles; // the first row tiles of a sequence that are split; later ones are not
     // splits > 1: of every part the rows [D], unnormalised and relative to their
     // maximum, by row and query head, then all (maximum, sum) pairs.
     float* partial;

@@ -492,6 +492,35 @@ def test_many_single_tokens_beside_a_chunk(gpu, fmt):
         assert cache.status() == A.KV_BAD_LENGTH
 
 
+@pytest.mark.parametrize("fmt,dtype", [("bf16", "bf16"), ("4bit", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("counts,lengths,heads,kv_heads,window", [
+    ([2150], [5500], 64, 64, 0), ([1500], [5500], 96, 32, 0), ([1700], [4500], 64, 64, 2100),
+    ([600, 480], [2700, 2500], 120, 40, 0)])
+def test_first_tiles_of_a_chunk_split(gpu, fmt, dtype, counts, lengths, heads, kv_heads, window):
+    """Somewhat more row tiles than the device takes at a time: the first ones, which
+    come last, are split. Rows beside every border of tiles, and others."""
+    dim, rng = 64, np.random.default_rng(49)
+    cache = M.Cache(fmt, lengths, kv_heads, dim, 64)
+    cache.upload()
+    q = new_rows(rng, [sum(counts)], heads, dim, dtype, std=2.0)
+    got = run_attention(cache, counts, q, dtype, window, 5, max_length=max(lengths))
+    again = run_attention(cache, counts, q, dtype, window, 5, max_length=max(lengths) // 2)
+    group, at = heads // kv_heads, 0
+    for s, n in enumerate(counts):
+        k, _ = cache.rows("k", s)
+        v, _ = cache.rows("v", s)
+        borders = {t * 128 // group + d for t in range(n * group // 128 + 1) for d in (-1, 0)}
+        for j in sorted({j for j in borders if 0 <= j < n} | {0, n - 1} | {int(x) for x in rng.integers(0, n, 20)}):
+            h = int(rng.integers(0, kv_heads))
+            end = lengths[s] - n + j + 1
+            want, bound = M.attention(q[at + j:at + j + 1, h * group:(h + 1) * group], k[:end, h:h + 1], v[:end, h:h + 1],
+                                      end, window, 5, 1, dim ** -0.5, dtype)
+            for x in (got, again):
+                assert (np.abs(x[at + j, h * group:(h + 1) * group] - want[0]) <= bound[0]).all(), (s, j, h)
+        at += n
+    assert cache.status() == 0
+
+
 def test_rows_bounds_above_the_rows(gpu):
     """max_rows as a bound: sequences may all be shorter."""
     rng = np.random.default_rng(46)
