@@ -201,8 +201,7 @@ def test_append_turns_as_mmrope(gpu):
     A.synchronize()
     index = plan.sequence_index()
     assert (np.sort(index) == np.arange(rows)).all()
-    np.testing.assert_allclose(out.read()[index, 0], dst.read()[:, 0][np.arange(rows)][...] if (index == np.arange(rows)).all()
-                               else dst.read()[:, 0], atol=4e-6 * 4)
+    np.testing.assert_allclose(out.read()[index, 0], dst.read()[:, 0], atol=4e-6 * 4)
 
 
 def test_append_four_bits_of_all_kinds(gpu):
@@ -668,6 +667,38 @@ def test_same_bits_every_time_and_on_another_stream(gpu):
         stream = A.Stream()
         for s in (None, stream):
             np.testing.assert_array_equal(run_attention(cache, counts, q, "bf16", stream=s), first)
+        stream.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["bf16", "4bit"])
+def test_in_place_and_two_calls_at_once(gpu, fmt, dtype):
+    """Queries become the output, on two streams side by side with a workspace each."""
+    rng = np.random.default_rng(50)
+    calls = []
+    for counts, lengths in ([1, 3, 1], [4000, 70, 9]), ([1, 260, 2], [5000, 800, 2]), ([300], [2000]):
+        cache = M.Cache(fmt, lengths, 2, 128, 16)
+        cache.upload()
+        q = new_rows(rng, counts, 6, 128, dtype)
+        calls.append((cache, counts, q, run_attention(cache, counts, q, dtype)))
+    streams = [A.Stream(), A.Stream()]
+    held = []
+    for _ in range(3):
+        for i, (cache, counts, q, _) in enumerate(calls):
+            rows = A.KvRows(max(counts), M_keep(np.cumsum([0] + counts)))
+            x = M.Rows(q, dtype)
+            n = A.kv_attention_workspace(cache.desc, rows, x.blob, A.KvMask())
+            held.append((i, x, A.DeviceBuffer(max(n, 16)), n, rows))
+    A.synchronize()
+    for j, (i, x, ws, n, rows) in enumerate(held):
+        A.kv_attention(calls[i][0].desc, rows, x.blob, A.KvMask(), 128 ** -0.5, x.blob, ws.ptr, n, streams[j % 2])
+    for stream in streams:
+        stream.synchronize()
+    for i, x, *_ in held:
+        np.testing.assert_array_equal(x.read(), calls[i][3])
+    for cache, counts, q, got in calls:
+        check_attention(cache, counts, q, dtype, got)
+    for stream in streams:
         stream.destroy()
 
 
