@@ -36,7 +36,8 @@ constexpr int kRowTile = 16;   // rows of kv_rows_kernel's tile
 constexpr int kTileRows = 128; // of kv_tile_kernel's
 constexpr int kKeyShift = 5;   // keys of both kernels' key tiles
 constexpr int kKeyTile = 1 << kKeyShift;
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;     // of kv_rows_kernel's workgroup
+constexpr int kWideWaves = 8; // where a CU has but one
 constexpr int kLongPart = 256; // key tiles of a part
 
 __device__ __forceinline__ float max_xor16(float x)
@@ -137,17 +138,18 @@ __device__ __forceinline__ bool some_row_sees(int key, const KvSpan& first, cons
     return key < last.end && (key + 16 > first.begin || key < last.sinks);
 }
 
-// One row tile of 16 rows, one part of its keys: each wave takes every fourth
-// key tile (32 keys) by itself, with K from memory straight into the MFMA
+// One row tile of 16 rows, one part of its keys: each of four (eight) waves takes
+// every fourth (eighth) key tile (32 keys) by itself, with K from memory straight into the MFMA
 // operand registers and V through the wave's own LDS, from which it is read
 // transposed; the waves' results are joined at the end. Bound by reading the
 // cache: the next tile's rows are asked for as soon as this one's registers are
 // free. One row over 131072 keys of 20 heads of 128, bf16: 227 us with the join,
 // 5.9 TB/s; 32 rows of up to 16384 keys over four bits 166 us, 5.0 TB/s, where
 // unpacking the codes shares the vector units with the softmax. (Eight or sixteen
-// waves a workgroup and registers for three or four workgroups a CU were slower,
-// as were chunks of V in an order that frees LDS of bank conflicts: 36.5 us to
-// 35.9 for bf16 rows of 16 sequences of 8000 keys, 31.2 to 32.3 for fp32 ones.)
+// waves a workgroup where CUs have several, and registers for three or four
+// workgroups of bf16 pages a CU were slower, as were chunks of V in an order that
+// frees LDS of bank conflicts: 36.5 us to 35.9 for bf16 rows of 16 sequences of
+// 8000 keys, 31.2 to 32.3 for fp32 ones.)
 //
 // S^T = K Q^T (16x16x32): lane (r = lane % 16, g = lane / 16) holds row r's
 // scores of keys 4 g + [0, 4) of each 16. Those of two blocks are, in that
@@ -155,8 +157,8 @@ __device__ __forceinline__ bool some_row_sees(int key, const KvSpan& first, cons
 // read in the same key order. Which features an MFMA takes of a row does not
 // matter as long as both operands agree: of 4-bit rows a lane has a quarter,
 // one load and one scale.
-template <int D, bool F32, bool FOUR>
-__global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionLaunch p)
+template <int D, bool F32, bool FOUR, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void kv_rows_kernel(const KvAttentionLaunch p)
 {
     constexpr int kPieces = F32 ? 3 : 1;
     constexpr int kChunks = D / 32;
@@ -165,8 +167,8 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     constexpr int kElem = F32 ? 4 : 2;
     constexpr int kVBytes = kKeyTile * kPitch * 2;
     constexpr int kOBytes = kRowTile * D * 4;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves][kVBytes > kOBytes ? kVBytes : kOBytes];
-    __shared__ float stats[kWaves][kRowTile][2];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[WAVES][kVBytes > kOBytes ? kVBytes : kOBytes];
+    __shared__ float stats[WAVES][kRowTile][2];
 
     const KvView& c = p.cache;
     const int seq = (blockIdx.y + blockIdx.z) % gridDim.y;
@@ -337,10 +339,10 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
         now = look_up(i);
         fetch_k(now);
         fetch_v(now);
-        next = look_up(min(i + kWaves, part_end - 1));
+        next = look_up(min(i + WAVES, part_end - 1));
     }
 #pragma unroll 1
-    for (; i < part_end; i += kWaves)
+    for (; i < part_end; i += WAVES)
     {
         const int key0 = now.key0;
         // Whether every row of the tile sees all its keys.
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
         const unsigned there = now.there;
         now = next;
         fetch_v(now);
-        next = look_up(min(i + 2 * kWaves, part_end - 1));
+        next = look_up(min(i + 2 * WAVES, part_end - 1));
 
         float x[8];
         float top = -INFINITY;
@@ -511,14 +513,14 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
         stats[wave][r][1] = row_sum;
     }
     __syncthreads();
-    constexpr int kPer = kRowTile * D / (kWaves * 64); // features a thread
+    constexpr int kPer = kRowTile * D / (WAVES * 64); // features a thread
     const int out_row = threadIdx.x * kPer / D;
     const int f0 = threadIdx.x * kPer % D;
     if (row0 + out_row > last)
         return;
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kWaves; i++)
+    for (int i = 0; i < WAVES; i++)
         m = fmaxf(m, stats[i][out_row][0]);
     const float from = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv_rows_kernel(const KvAttentionL
     for (int e = 0; e < kPer; e++)
         v[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWaves; i++)
+    for (int i = 0; i < WAVES; i++)
     {
         if (stats[i][out_row][0] == -INFINITY)
             continue;
@@ -1487,7 +1489,20 @@ void kv_attention_deal(KvAttentionLaunch& p, int max_length)
                 splits = n;
             }
         }
-        p.one = p.more = parts(splits);
+        // About a workgroup a CU: eight waves read as much as several workgroups of
+        // four, without parts to join. Below the given key tiles; one token each, us
+        // split and so: 120 workgroups over 1000 keys, bf16 20.6, 18.1, four bits
+        // 17.3, 14.2; over 8000 92, 104 and 37, 53; 160 over 2000 33.5, 29.5 and 22,
+        // 20.5; over 8000 117, 114 and 47, 53; 240 over 2000 44, 40 and 26, 22; over
+        // 8000 170, 167 and 59, 56; 100 over 1000 18.6, 17.7 and 15.8, 13.5, over 4000
+        // 39, 43 and 24, 29.
+        const long long most = blocks < 80 || blocks > 256 ? 0
+                               : blocks < 112              ? 45
+                               : blocks < 144              ? (p.four ? 50 : 150)
+                               : blocks < 224              ? (p.four ? 100 : 256)
+                                                           : 256;
+        p.wide = splits > 1 && count <= most;
+        p.one = p.more = parts(p.wide ? 1 : splits);
         return;
     }
     // (Without a window the rows of a chunk see, on the average, all but half of it.)
@@ -1634,7 +1649,10 @@ hipError_t launch(const KvAttentionLaunch& p, hipStream_t stream)
     if (p.few)
     {
         const dim3 grid(p.tiles * p.cache.heads, p.cache.sequences, p.one.splits);
-        hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR>), grid, dim3(kWaves * 64), 0, stream, p);
+        if (p.wide)
+            hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR, kWideWaves>), grid, dim3(kWideWaves * 64), 0, stream, p);
+        else
+            hipLaunchKernelGGL((kv_rows_kernel<D, F32, FOUR, kWaves>), grid, dim3(kWaves * 64), 0, stream, p);
     }
     else
     {

@@ -196,6 +196,7 @@ struct KvAttentionLaunch
     KvMaskRule mask;
     float scale_log2; // softmax scale * log2 e
     bool few;         // rows: row tiles of 16, else of 128
+    bool wide;        // few: eight waves a workgroup, not four
     int tiles;        // row tiles of the longest sequence
     // Of sequences of one tile of 128 rows, and of longer ones.
     KvParts one, more;
