@@ -520,6 +520,24 @@ def test_first_tiles_of_a_chunk_split(gpu, fmt, dtype, counts, lengths, heads, k
     assert cache.status() == 0
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["bf16", "4bit"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (900, 33)])
+def test_about_a_workgroup_a_cu(gpu, dtype, fmt, dim, window, sinks):
+    """Single and draft tokens of a batch whose heads are about as many as CUs."""
+    rng = np.random.default_rng(51)
+    counts = [int(x) for x in rng.choice([0, 1, 1, 2], 60)]
+    lengths = [c + int(x) for c, x in zip(counts, rng.integers(0, 1200, 60))]
+    cache = M.Cache(fmt, lengths, 2, dim, 32)
+    cache.upload()
+    q = new_rows(rng, [sum(counts)], 4, dim, dtype, std=2.0)
+    for bound in (max(lengths), 1100):
+        got = run_attention(cache, counts, q, dtype, window, sinks, max_length=bound)
+        check_attention(cache, counts, q, dtype, got, window, sinks)
+    assert cache.status() == 0
+
+
 def test_rows_bounds_above_the_rows(gpu):
     """max_rows as a bound: sequences may all be shorter."""
     rng = np.random.default_rng(46)
